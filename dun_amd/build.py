@@ -36,7 +36,10 @@ def build_library(force=False, verbose=False):
     headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "depth_finalize.h"), os.path.join(HERE, "..", "include", "dun_hip.h")]
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    flags = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function"]
+    # packed fp32 instructions off: some of their forms have given wrong results on this hardware now and then (the host
+    # pass warns that it does not know the feature)
+    flags = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     jobs = []
     objs = []
     for src in SOURCES:
