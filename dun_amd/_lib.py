@@ -25,9 +25,13 @@ EXPORTS = [
     "dun_sgd_step_multi", "dun_sgd_step_multi_gated", "dun_label_count_bad", "dun_predict_gauss_step", "dun_fc_small_net_mode", "dun_fc_sync_bytes", "dun_fc_sync_status",
     "dun_fc_objective_in_forward", "dun_fc_head_grads_in_forward", "dun_copy_pair",
     "dun_copy_pair_indirect", "dun_predict_gauss_step_signal", "dun_gemm_profile_begin", "dun_gemm_profile_end",
+    "dun_layer_norm_forward", "dun_layer_norm_backward_workspace_floats", "dun_layer_norm_backward", "dun_act8_pack",
+    "dun_act8_unpack", "dun_act8_weight_grad_workspace_floats", "dun_act8_weight_grad",
 ]
 
 SGD_MAX_SEGMENTS = 24
+ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DUN_F32, DUN_BF16, DUN_F16
+ACT8_GROUP = 32
 
 
 def res_floats(D):
@@ -87,7 +91,7 @@ _lib = None
 
 
 def _declare(lib):
-    vp, i, f, d, sz = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_size_t
+    vp, i, f, d, sz, ll = C.c_void_p, C.c_int, C.c_float, C.c_double, C.c_size_t, C.c_int64
     sig = {
         "dun_abi_version": (i, []),
         "dun_last_error": (C.c_char_p, []),
@@ -142,6 +146,13 @@ def _declare(lib):
         "dun_gemm_profile_begin": (i, [i]),
         "dun_gemm_profile_end": (i, [C.POINTER(GemmProfileRec), i]),
         "dun_copy_pair_indirect": (i, [vp, sz, vp, sz, vp, vp]),
+        "dun_layer_norm_forward": (i, [vp, ll, vp, ll, vp, vp, vp, ll, vp, vp, vp, vp, vp, ll, i, i, f, i, vp]),
+        "dun_layer_norm_backward_workspace_floats": (sz, [ll, i, i, i]),
+        "dun_layer_norm_backward": (i, [vp, ll, vp, ll, vp, vp, vp, vp, vp, ll, vp, i, vp, sz, ll, i, i, i, vp]),
+        "dun_act8_pack": (i, [vp, ll, vp, vp, ll, i, i, i, vp]),
+        "dun_act8_unpack": (i, [vp, vp, vp, ll, ll, i, i, i, vp]),
+        "dun_act8_weight_grad_workspace_floats": (sz, [ll, i, i, i]),
+        "dun_act8_weight_grad": (i, [vp, ll, vp, vp, vp, vp, vp, sz, ll, i, i, i, i, vp]),
         "dun_predict_gauss_step_signal": (i, [vp, vp, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     }
     for name, (res, args) in sig.items():
@@ -202,3 +213,34 @@ def out_ptr(t):
         raise RuntimeError("dun_amd kernels write to GPU tensors or contiguous pinned host tensors")
     return t.data_ptr()
 
+
+
+class _Nothing(object):
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_NOTHING = _Nothing()
+
+
+def on_device(t):
+    """Context in which `t`'s device is the current one (kernels launch on the current device)."""
+    if not t.is_cuda:
+        raise RuntimeError("dun_amd kernels need GPU tensors (got a %s tensor); there is no CPU path" % t.device)
+    if t.device.index == torch.cuda.current_device():
+        return _NOTHING
+    return torch.cuda.device(t.device)
+
+
+def rows_view(t):
+    """(tensor, row stride) of a 2-D tensor whose rows the kernels can walk: unit column stride, rows that do not overlap;
+    anything else (transposed, expanded) is copied."""
+    rows, cols = t.shape
+    ld = t.stride(0)
+    if (t.stride(1) == 1 or cols == 1) and (ld >= cols or rows <= 1):
+        return t, (ld if rows > 1 else cols)
+    t = t.contiguous()
+    return t, cols

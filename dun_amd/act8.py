@@ -1,0 +1,146 @@
+"""8-bit activation checkpoints and the gradients that are taken from them.
+
+A training step keeps every layer's input for its backward.  ``pack`` keeps it in 1 + 1/32 bytes per element: 8-bit codes and one
+power-of-two scale per 32 consecutive columns of a row,
+
+    value = code * 2^e,   e the smallest integer (not below -126) for which the group's largest magnitude rounds to at
+                          most 127 (255 for a rectified input, ``relu=True``: unsigned codes of max(x, 0)),
+
+rounded to nearest even, so an element is off by at most half a step and a step is at most the group's largest magnitude / 63.75
+(127.75 rectified).  A positive element of a rectified input keeps a code of at least 1: ``value > 0`` is ReLU's mask.
+A group that holds an infinity or a NaN, or whose largest magnitude would round to 2^128, reads back as NaN.
+
+``weight_grad`` takes a Linear layer's weight gradient straight from the codes: a value is a bf16 number, an fp32
+gradient the exact sum of three, so the product runs on the bf16 matrix cores without losing a bit of its operands.
+``linear`` / ``Linear`` is the layer whose backward does so (float32, the framework's own products either way).
+
+No counterpart in the reference, which keeps everything in float32.
+"""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib as L
+from . import kernels
+
+
+def _as_rows(t, what):
+    """[..., cols] as a 2-D tensor of rows."""
+    if not isinstance(t, torch.Tensor) or t.dim() < 1:
+        raise RuntimeError("%s must be a tensor of at least one dimension" % what)
+    if t.dtype not in L.ROW_DTYPES:
+        raise RuntimeError("%s must be float32, bfloat16 or float16 (got %s)" % (what, t.dtype))
+    if t.shape[-1] == 0:
+        raise RuntimeError("%s has rows of no elements: %s" % (what, tuple(t.shape)))
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+class Packed8(object):
+    """An 8-bit checkpoint of a tensor: ``codes`` uint8 [rows, 32 G] (signed codes are stored + 128) and ``exps`` uint8
+    [rows, G] (exponents + 127), G = ceil(cols / 32)."""
+    __slots__ = ("codes", "exps", "shape", "relu", "dtype")
+
+    def __init__(self, codes, exps, shape, relu, dtype):
+        self.codes, self.exps, self.shape, self.relu, self.dtype = codes, exps, tuple(shape), bool(relu), dtype
+        cols = self.shape[-1]
+        groups = (cols + L.ACT8_GROUP - 1) // L.ACT8_GROUP
+        rows = 1
+        for n in self.shape[:-1]:
+            rows *= n
+        for t, want in ((codes, (rows, groups * L.ACT8_GROUP)), (exps, (rows, groups))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != want or not t.is_contiguous() or t.device != codes.device:
+                raise RuntimeError("not a checkpoint of a tensor of shape %s: uint8 %s wanted, got %s %s"
+                                   % (self.shape, want, t.dtype, tuple(t.shape)))
+
+    @property
+    def packed(self):
+        return self.codes, self.exps
+
+    @property
+    def nbytes(self):
+        return self.codes.numel() + self.exps.numel()
+
+    def unpack(self, dtype=torch.float32):
+        """The values that the codes stand for (exact in float32 and bfloat16)."""
+        if dtype not in L.ROW_DTYPES:
+            raise RuntimeError("a checkpoint unpacks to float32, bfloat16 or float16 (got %s)" % dtype)
+        return kernels.backend().act8_unpack(self.packed, self.shape[-1], self.relu, dtype).view(self.shape)
+
+
+def pack(x, relu=False):
+    """The 8-bit checkpoint of ``x`` [..., cols], or of max(x, 0) with ``relu``."""
+    x2 = _as_rows(x.detach(), "pack: x")
+    codes, exps = kernels.backend().act8_pack(x2, bool(relu))
+    return Packed8(codes, exps, x.shape, relu, x.dtype)
+
+
+def weight_grad(dy, packed, bias=True):
+    """(dw [outs, cols], db [outs]): the float32 gradients of the weight and bias of a Linear layer, from the gradient
+    ``dy`` [..., outs] of its output and the checkpoint of its input.  ``bias=False``: db is None."""
+    if not isinstance(packed, Packed8):
+        raise RuntimeError("weight_grad: packed must be a Packed8 (got %s)" % type(packed).__name__)
+    dy2 = _as_rows(dy.detach(), "weight_grad: dy")
+    if tuple(dy.shape[:-1]) != packed.shape[:-1] or dy.device != packed.codes.device:
+        raise RuntimeError("weight_grad: dy %s on %s does not belong to a checkpoint of %s on %s"
+                           % (tuple(dy.shape), dy.device, packed.shape, packed.codes.device))
+    return kernels.backend().act8_weight_grad(dy2, packed.packed, packed.shape[-1], packed.relu, want_bias=bool(bias))
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, packed):
+        be = kernels.backend()
+        x2 = x.detach().reshape(-1, x.shape[-1]).contiguous()
+        w = weight.detach().contiguous()
+        rows, cols, outs = x2.shape[0], x2.shape[1], w.shape[0]
+        ctx.shape, ctx.has_bias, ctx.relu = tuple(x.shape), bias is not None, False
+        codes = exps = None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            codes, exps = be.act8_pack(x2, False) if packed is None else packed.packed
+            ctx.relu = False if packed is None else packed.relu
+        ctx.save_for_backward(weight, codes, exps)
+        if rows == 0:
+            return x.new_empty(x.shape[:-1] + (outs,))
+        with L.on_device(x2):
+            y = be.gemm(x2, w, rows, outs, cols, bias=None if bias is None else bias.detach().contiguous())
+        return y.view(x.shape[:-1] + (outs,))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        be = kernels.backend()
+        weight, codes, exps = ctx.saved_tensors
+        outs, cols = weight.shape
+        dy2 = dy.reshape(-1, outs).contiguous()
+        dx = dw = db = None
+        if ctx.needs_input_grad[0]:
+            if dy2.shape[0] == 0:
+                dx = dy.new_empty(ctx.shape)
+            else:
+                with L.on_device(dy2):
+                    dx = be.gemm(dy2, weight.detach().contiguous(), dy2.shape[0], cols, outs, b_kcontig=False).view(ctx.shape)
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dw, db = be.act8_weight_grad(dy2, (codes, exps), cols, ctx.relu, want_bias=ctx.has_bias)
+        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None
+
+
+def linear(x, weight, bias=None, packed=None):
+    """x weight^T + bias, like torch.nn.functional.linear, keeping ``x`` for the backward in 8 bits.  ``packed``: the
+    checkpoint of ``x`` where the caller has it already (layer_norm's ``pack_output``).  float32."""
+    for t, what in ((x, "x"), (weight, "weight"), (bias, "bias")):
+        if t is not None and (t.dtype != torch.float32 or t.device != x.device):
+            raise RuntimeError("linear: %s must be float32 on %s (got %s on %s)" % (what, x.device, t.dtype, t.device))
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        raise RuntimeError("linear: x %s does not go with weight %s" % (tuple(x.shape), tuple(weight.shape)))
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise RuntimeError("linear: bias %s does not go with weight %s" % (tuple(bias.shape), tuple(weight.shape)))
+    if packed is not None and (not isinstance(packed, Packed8) or packed.shape != tuple(x.shape) or packed.codes.device != x.device):
+        raise RuntimeError("linear: packed is not a checkpoint of x %s" % (tuple(x.shape),))
+    return _Linear8.apply(x, weight, bias, packed)
+
+
+class Linear(nn.Linear):
+    """nn.Linear that keeps its input for the backward in 8 bits; same parameters and state_dict."""
+
+    def forward(self, x, packed=None):
+        return linear(x, self.weight, self.bias, packed)

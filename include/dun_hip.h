@@ -425,6 +425,56 @@ int dun_copy_pair(void* dst0, const void* src0, size_t bytes0, void* dst1, const
 int dun_copy_pair_indirect(void* dst0, size_t bytes0, void* dst1, size_t bytes1, const void* const* src_table,
                            dun_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------------
+ * Layer normalisation over rows, and 8-bit activation checkpoints.  NO COUNTERPART IN THE REFERENCE, whose blocks know
+ * BatchNorm only (src/DUN/layers.py:33-53): the residual trunk with LayerNorm blocks
+ * (dun_amd.stochastic_fc_models.arq_uncert_fc_resnet_ln) runs on these.
+ * Rows are row-major with a stride in ELEMENTS (>= cols); `dtype` names the type of x, res, y, dy and dx, everything else
+ * is fp32.  Pointers need the alignment of their element, codes 8 bytes.  rows == 0 is allowed.
+ *
+ * The 8-bit checkpoint of [rows, cols]: codes [rows, 32 G] and exps [rows, G], G = ceil(cols / 32).
+ *   value(r, c) = (codes[r, c] - zero) * 2^(exps[r, c / 32] - 127), zero = 128, or 0 for a rectified input
+ * with the smallest power of two, not below 2^-126, for which the group's largest magnitude rounds to at most 127
+ * (255 rectified); codes round to nearest even; a positive element of a rectified input keeps a code >= 1; codes past
+ * `cols` are zero.  A group that holds an infinity or a NaN, or whose largest magnitude would round to 2^128, has exps 255
+ * and reads back as NaN.
+ * ---------------------------------------------------------------------------------------------------- */
+#define DUN_F32 0
+#define DUN_BF16 1
+#define DUN_F16 2
+
+/* z = x, or max(x, 0) with relu; y = [res +] (z - mean) / sqrt(var + eps) * w + b over each row (biased variance).
+ * w, b [cols], each nullable (1, 0).  stats float [2][rows] (nullable): mean, 1 / sqrt(var + eps), what backward needs.
+ * x_codes / x_exps (nullable): the checkpoint of z, rectified with relu; y_codes / y_exps (nullable): of y, signed. */
+int dun_layer_norm_forward(const void* x, int64_t ldx, const void* res, int64_t ldr, const float* w, const float* b, void* y,
+                           int64_t ldy, float* stats, uint8_t* x_codes, uint8_t* x_exps, uint8_t* y_codes, uint8_t* y_exps,
+                           int64_t rows, int cols, int dtype, float eps, int relu, dun_stream_t stream);
+/* Backward from x or from its checkpoint (the other NULL), with the forward's stats: dx (may be dy itself; the residual's
+ * gradient is dy), and with sums 2 or 3 the column sums sums_out float [sums][cols]: sum dy xhat (the gradient of w),
+ * sum dy (of b), and with 3 sum dx (of the bias of the Linear that made x).  ws: scratch of
+ * dun_layer_norm_backward_workspace_floats() floats.  The sums are added in a fixed order: the same bits every time. */
+size_t dun_layer_norm_backward_workspace_floats(int64_t rows, int cols, int dtype, int sums);
+int dun_layer_norm_backward(const void* dy, int64_t lddy, const void* x, int64_t ldx, const uint8_t* x_codes,
+                            const uint8_t* x_exps, const float* w, const float* stats, void* dx, int64_t lddx,
+                            float* sums_out, int sums, float* ws, size_t ws_floats, int64_t rows, int cols, int dtype,
+                            int relu, dun_stream_t stream);
+
+/* The checkpoint of x by itself, and back to values (of `dtype`). */
+int dun_act8_pack(const void* x, int64_t ldx, uint8_t* codes, uint8_t* exps, int64_t rows, int cols, int dtype, int relu,
+                  dun_stream_t stream);
+int dun_act8_unpack(const uint8_t* codes, const uint8_t* exps, void* out, int64_t ldo, int64_t rows, int cols, int dtype,
+                    int relu, dun_stream_t stream);
+/* A Linear layer's gradients with its input taken from the checkpoint (rows, cols, relu: the checkpoint's):
+ * dw float [outs, cols] = dy^T value, db float [outs] (nullable) = sum_rows dy; dy [rows, outs] of `dtype`, stride lddy.
+ * A value has at most 8 significant bits and a power-of-two scale, hence is a bf16 number; dy is taken apart into bf16
+ * numbers (fp32: three, fp16: two, bf16: one) whose sum it is; the products are exact and accumulate in fp32 on the bf16 matrix
+ * cores.  (Parts of dy below 2^-133 are lost.  A non-finite dy gives a non-finite, not necessarily the same, result.)
+ * ws: scratch of dun_act8_weight_grad_workspace_floats() floats. */
+size_t dun_act8_weight_grad_workspace_floats(int64_t rows, int outs, int cols, int dtype);
+int dun_act8_weight_grad(const void* dy, int64_t lddy, const uint8_t* codes, const uint8_t* exps, float* dw, float* db,
+                         float* ws, size_t ws_floats, int64_t rows, int outs, int cols, int dtype, int relu,
+                         dun_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
