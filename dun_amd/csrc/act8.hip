@@ -14,17 +14,17 @@
 
 namespace dun {
 
-typedef u32 u32x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef u32 u32x4_any __attribute__((ext_vector_type(4), aligned(8)));
 typedef u32 u32_any __attribute__((aligned(2)));
-typedef u32 u32x2_any __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
 
 // ---- pack / unpack: elementwise streams -----------------------------------------------------------------------------------------
 // One vector of E columns per lane; a row is G * 32 / E vectors (padded groups included), so the lanes of a group are neighbours.
 template <typename T>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T* x, size_t ldx, uint8_t* codes, uint8_t* exps, size_t vecs,
                                                         u32 vpr, int cols, int relu) {
-    constexpr int E = Row<T>::E, GV = ACT8_GROUP / E;
+    constexpr int GV = ACT8_GROUP / E;
     for (size_t v0 = (size_t)blockIdx.x * 256; v0 < vecs; v0 += (size_t)gridDim.x * 256) {
         const size_t i = v0 + threadIdx.x;
         if (i >= vecs) break;  // (vecs is a multiple of GV: the lanes of a group stay together)
@@ -43,9 +43,9 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const T* x, size_t ldx, 
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = rectify(v[e]);
         }
-        u32 w[E / 4];
-        const u32 byte = act8_pack<E>(v, relu, w);
-        act8_store_words<E>(codes + i * E, w);
+        u32 byte;
+        const u32 word = act8_pack(v, relu, &byte);
+        *reinterpret_cast<u32*>(codes + i * E) = word;
         if (vec % GV == 0) exps[i / GV] = (uint8_t)byte;
     }
 }
@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void act8_pack_kernel(const T* x, size_t ldx, 
 template <typename T>
 __global__ __launch_bounds__(256) void act8_unpack_kernel(const uint8_t* codes, const uint8_t* exps, T* out, size_t ldo,
                                                           size_t vecs, u32 vpr, int cols, float zero) {
-    constexpr int E = Row<T>::E, GV = ACT8_GROUP / E;
+    constexpr int GV = ACT8_GROUP / E;
     for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < vecs; i += (size_t)gridDim.x * 256) {
         size_t row;
         u32 vec;
@@ -64,10 +64,8 @@ __global__ __launch_bounds__(256) void act8_unpack_kernel(const uint8_t* codes, 
             row = i / vpr;
             vec = (u32)(i - row * vpr);
         }
-        u32 w[E / 4];
         float v[E];
-        act8_load_words<E>(codes + i * E, w);
-        act8_values<E>(w, exps[i / GV], zero, v);
+        act8_values(*reinterpret_cast<const u32*>(codes + i * E), exps[i / GV], zero, v);
         store_part(out + row * ldo, (int)vec * E, cols, v);
     }
 }
@@ -77,9 +75,9 @@ struct WgradP {
     const void* dy;
     const uint8_t* codes;
     const uint8_t* exps;
-    float* dw;  // [S][O][I]
-    float* db;  // [S][O] or null
-    size_t lddy, rows;
+    float* dw;  // [S][O][I], `stride` apart
+    float* db;  // [S][O], `stride` apart, or null
+    size_t lddy, rows, stride;
     size_t rows_per;  // rows of one split, a multiple of 32
     int O, I, groups, pitch;
     int tiles_m, tiles_n, splits;
@@ -117,89 +115,457 @@ __device__ __forceinline__ float code_value(u32 word, int j, float s, float zero
     return ((float)((word >> (8 * j)) & 0xffu) - zero) * s;
 }
 
-// Simplest form: one wave per 32 x 32 tile of dw and split, operands from global memory straight into MFMA registers.
-// v_mfma_f32_32x32x16_bf16: lane l holds row / column l % 32 and reduction indices 8 (l / 32) .. + 7.
-template <typename T>
-__global__ __launch_bounds__(64) void act8_wgrad_simple_kernel(const WgradP p) {
-    constexpr int N = Terms<T>::N;
-    const int lane = threadIdx.x, c = lane & 31, kc = lane >> 5;
+// What a thread holds of dy between its load and the matrix cores: AC neighbouring columns of 8 rows
+template <typename T, int AC> struct DyRegs {
+    float v[8][AC];
+    __device__ __forceinline__ void get(int j, const float* p) {
+        if constexpr (AC == 2) {
+            const f32x2_any q = *reinterpret_cast<const f32x2_any*>(p);
+            v[j][0] = q[0];
+            v[j][1] = q[1];
+        } else {
+            v[j][0] = *p;
+        }
+    }
+    __device__ __forceinline__ void get1(int j, int c, const float* p) { v[j][c] = *p; }
+    __device__ __forceinline__ void clear(int j) {
+#pragma unroll
+        for (int c = 0; c < AC; ++c) v[j][c] = 0.f;
+    }
+    __device__ __forceinline__ float value(int j, int c) const { return v[j][c]; }
+    __device__ __forceinline__ void terms(int c, u32x4_t* out) const {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = v[j][c];
+        split_terms<3>(x, out);
+    }
+};
+template <typename T, int AC> struct DyRegs16 {
+    u32 v[8];  // AC = 2: both columns in a word
+    __device__ __forceinline__ void get(int j, const T* p) {
+        if constexpr (AC == 2) {
+            v[j] = *reinterpret_cast<const u32_any*>(p);
+        } else {
+            v[j] = p->bits;
+        }
+    }
+    __device__ __forceinline__ void get1(int j, int c, const T* p) {
+        v[j] = c == 0 ? (u32)p->bits : (v[j] & 0xffffu) | ((u32)p->bits << 16);
+    }
+    __device__ __forceinline__ void clear(int j) { v[j] = 0; }
+    __device__ __forceinline__ float value(int j, int c) const { return to_f32(T{(u16)(v[j] >> (16 * c))}); }
+};
+template <int AC> struct DyRegs<bf16_t, AC> : DyRegs16<bf16_t, AC> {
+    __device__ __forceinline__ void terms(int c, u32x4_t* out) const {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            out[0][q] = __builtin_amdgcn_perm(this->v[2 * q + 1], this->v[2 * q], c ? 0x07060302u : 0x05040100u);
+    }
+};
+template <int AC> struct DyRegs<fp16_t, AC> : DyRegs16<fp16_t, AC> {
+    __device__ __forceinline__ void terms(int c, u32x4_t* out) const {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = this->value(j, c);
+        split_terms<2>(x, out);
+    }
+};
+
+// Barrier for data in LDS only: loads from global memory stay in flight across it
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// A workgroup owns a BM x BN tile of dw over one range of rows and walks it 32 rows at a time through two LDS buffers of
+// bf16 operands: [column][32 rows], 64 bytes a column, N such planes for dy and one for the values.  While the matrix
+// cores work on one buffer, the rows two steps ahead are on their way into registers and those one step ahead are taken
+// apart into the other buffer.  Waves own WM x WN sub-tiles; dy has N planes, so WM < WN keeps the LDS reads of a wave, N WM + WN
+// columns per step, low.
+// A column's four 16-byte chunks (8 rows each) and the column's place among its neighbours are permuted by its
+// index so that the writes (columns 1, 2 or 4 apart, one chunk) and the reads (columns in a row, one chunk) spread over the banks.
+__device__ __forceinline__ int lds_chunk(int col, int kc) {
+    const int a = (col >> 2) & 3;
+    return ((col & ~3) | ((col & 3) ^ a)) * 4 + (kc ^ a ^ ((col >> 4) & 3));
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) >= 8 ? 2 : 1) void act8_wgrad_tile_kernel(const WgradP p) {
+    constexpr int N = Terms<T>::N, NT = (BM / WM) * (BN / WN) * 64;
+    constexpr int AC = 4 * BM / NT, BC = 8 * BN / NT;
+    constexpr int MT = WM / 32, CT = WN / 32;
+    constexpr int PLANE_A = BM * 4, PLANE_B = BN * 4;  // 16-byte chunks
+    constexpr int BUF = N * PLANE_A + PLANE_B;
+    __shared__ u32x4_t lds[2 * BUF];
+
+    // workgroups go round-robin over the 8 XCDs: each takes a contiguous range of (split, tile row, tile column), so that the
+    // tiles that read the same rows of dy and codes meet in one L2
     int id = blockIdx.x;
+    {
+        const int nwg = gridDim.x, q = nwg >> 3, r = nwg & 7, xcd = id & 7, idx = id >> 3;
+        id = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+    }
     const int tn = id % p.tiles_n;
     id /= p.tiles_n;
     const int tm = id % p.tiles_m, split = id / p.tiles_m;
-    const int o = tm * 32 + c, i = tn * 32 + c;
+    const int m0 = tm * BM, n0 = tn * BN;
     const size_t r_begin = (size_t)split * p.rows_per;
     const size_t r_end = r_begin + p.rows_per < p.rows ? r_begin + p.rows_per : p.rows;
-    const T* dy = (const T*)p.dy;
-    f32x16 acc;
+    const int steps = (int)((r_end - r_begin + 31) / 32);
+
+    const int tid = threadIdx.x;
+    // dy: 8 rows x AC columns.  Columns past the last are read from the last: they make rows of dw that nobody stores.
+    const int a_cg = tid % (BM / AC), a_kc = tid / (BM / AC);
+    const bool m_full = m0 + BM <= p.O;
+    // (addresses: a base that is the same for all lanes, plus a 32-bit offset of the lane that never changes)
+    u32 a_off[AC];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0.f;
-    float bias = 0.f;
-    for (size_t r0 = r_begin; r0 < r_end; r0 += 16) {
-        float a[8], b[8];
+    for (int c = 0; c < AC; ++c) {
+        const int o = m0 + a_cg * AC + c;
+        a_off[c] = (u32)(a_kc * 8 * (u32)p.lddy + (o < p.O ? o : p.O - 1)) * (u32)sizeof(T);
+    }
+    const char* a_base = (const char*)p.dy + r_begin * p.lddy * sizeof(T);
+    const u32 a_row = (u32)p.lddy * (u32)sizeof(T);
+    // codes: 4 rows x BC columns, one group
+    const int b_cg = tid % (BN / BC), b_kq = tid / (BN / BC);
+    int b_col = n0 + b_cg * BC;
+    b_col = b_col < p.pitch ? b_col : p.pitch - BC;
+    const u32 b_off = (u32)(b_kq * 4) * (u32)p.pitch + (u32)b_col;
+    const u32 e_off = (u32)(b_kq * 4) * (u32)p.groups + (u32)(b_col / ACT8_GROUP);
+    const uint8_t* b_base = p.codes + r_begin * p.pitch;
+    const uint8_t* e_base = p.exps + r_begin * p.groups;
+
+    DyRegs<T, AC> ra;
+    u32 rb[4], re[4];
+    auto get_a = [&](int j, int c) { return (const T*)(a_base + (size_t)j * a_row + a_off[c]); };
+    auto get_b = [&](int j) {
+        const uint8_t* q = b_base + (size_t)j * p.pitch + b_off;
+        return BC == 4 ? *reinterpret_cast<const u32*>(q) : (u32)*reinterpret_cast<const u16*>(q);
+    };
+    auto get_e = [&](int j) { return (u32)*(e_base + (size_t)j * p.groups + e_off); };
+    auto load = [&](int step) {
+        const size_t left = r_end - r_begin - (size_t)step * 32;
+        if (left >= 32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const size_t r = r0 + kc * 8 + j;
-            const bool in = r < r_end;
-            a[j] = in && o < p.O ? to_f32(dy[r * p.lddy + o]) : 0.f;
-            const bool inb = in && i < p.pitch;
-            const u32 code = inb ? p.codes[r * p.pitch + i] : 0u;
-            const float s = inb ? act8_scale(p.exps[r * p.groups + i / ACT8_GROUP]) : 0.f;
-            b[j] = code_value(code, 0, s, inb ? p.zero : 0.f);
-            bias += a[j];
+            for (int j = 0; j < 4; ++j) {
+                rb[j] = get_b(j);
+                re[j] = get_e(j);
+            }
+            if (m_full) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) ra.get(j, get_a(j, 0));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int c = 0; c < AC; ++c) ra.get1(j, c, get_a(j, c));
+            }
+        } else {  // rows past the last are zeros in both operands (a value there could be a NaN)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                ra.clear(j);
+                if ((size_t)(a_kc * 8 + j) < left) {
+#pragma unroll
+                    for (int c = 0; c < AC; ++c) ra.get1(j, c, get_a(j, c));
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                rb[j] = p.zero != 0.f ? 0x80808080u : 0u;
+                re[j] = 0;
+                if ((size_t)(b_kq * 4 + j) < left) {
+                    rb[j] = get_b(j);
+                    re[j] = get_e(j);
+                }
+            }
         }
-        u32x4_t at[N], bt[1];
-        split_terms<N>(a, at);
-        split_terms<1>(b, bt);
+        a_base += (size_t)32 * a_row;
+        b_base += (size_t)32 * p.pitch;
+        e_base += (size_t)32 * p.groups;
+    };
+
+    const bool want_db = p.db && tn == 0;
+    double bias[AC];
 #pragma unroll
-        for (int t = 0; t < N; ++t)
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, at[t]), __builtin_bit_cast(bf16x8_t, bt[0]), acc, 0, 0, 0);
-    }
-    float* dw = p.dw + (size_t)split * p.O * p.I;
+    for (int c = 0; c < AC; ++c) bias[c] = 0.0;
+    auto stage = [&](int buf) {
+        u32x4_t* A = lds + buf * BUF;
+        u32x4_t* B = A + N * PLANE_A;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        const int m = tm * 32 + (e & 3) + 8 * (e >> 2) + 4 * kc;
-        if (m < p.O && i < p.I) dw[(size_t)m * p.I + i] = acc[e];
+        for (int c = 0; c < AC; ++c) {
+            u32x4_t t[N];
+            ra.terms(c, t);
+            const int at = lds_chunk(a_cg * AC + c, a_kc);
+#pragma unroll
+            for (int k = 0; k < N; ++k) A[k * PLANE_A + at] = t[k];
+        }
+        if (want_db) {
+#pragma unroll
+            for (int c = 0; c < AC; ++c) {
+                const float s0 = ra.value(0, c) + ra.value(1, c), s1 = ra.value(2, c) + ra.value(3, c);
+                const float s2 = ra.value(4, c) + ra.value(5, c), s3 = ra.value(6, c) + ra.value(7, c);
+                bias[c] += (double)((s0 + s1) + (s2 + s3));
+            }
+        }
+        float s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = act8_scale(re[j]);
+#pragma unroll
+        for (int c = 0; c < BC; ++c) {
+            u32x2_t w;
+            w[0] = top_halves(code_value(rb[1], c, s[1], p.zero), code_value(rb[0], c, s[0], p.zero));
+            w[1] = top_halves(code_value(rb[3], c, s[3], p.zero), code_value(rb[2], c, s[2], p.zero));
+            reinterpret_cast<u32x2_t*>(B)[lds_chunk(b_cg * BC + c, b_kq >> 1) * 2 + (b_kq & 1)] = w;
+        }
+    };
+
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = (wave / (BN / WN)) * WM, wn = (wave % (BN / WN)) * WN;
+    const int fc = lane & 31, fk = lane >> 5;
+    f32x16 acc[MT][CT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    auto compute = [&](int buf) {
+        const u32x4_t* A = lds + buf * BUF;
+        const u32x4_t* B = A + N * PLANE_A;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            u32x4_t b[CT];
+#pragma unroll
+            for (int j = 0; j < CT; ++j) b[j] = B[lds_chunk(wn + 32 * j + fc, 2 * ks + fk)];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int at = lds_chunk(wm + 32 * i + fc, 2 * ks + fk);
+                u32x4_t a[N];
+#pragma unroll
+                for (int t = 0; t < N; ++t) a[t] = A[t * PLANE_A + at];
+#pragma unroll
+                for (int t = 0; t < N; ++t)
+#pragma unroll
+                    for (int j = 0; j < CT; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[t]), __builtin_bit_cast(bf16x8_t, b[j]),
+                                                                            acc[i][j], 0, 0, 0);
+            }
+        }
+    };
+
+    // Two waves share a SIMD in the large tile: one of each pair takes its rows apart before its matrix products, the other after them, so
+    // that the vector and the matrix pipe both have work all the time.
+    const bool early = NT >= 512 && wave < NT / 128;
+    load(0);
+    stage(0);
+    if (steps > 1) load(1);
+    lds_barrier();
+    for (int k = 0; k < steps; ++k) {
+        const bool more = k + 1 < steps;
+        if (early && more) {
+            stage((k + 1) & 1);
+            if (k + 2 < steps) load(k + 2);
+        }
+        compute(k & 1);
+        if (!early && more) {
+            stage((k + 1) & 1);
+            if (k + 2 < steps) load(k + 2);
+        }
+        lds_barrier();
     }
-    if (p.db && tn == 0) {
-        bias += __shfl_xor(bias, 32, 64);
-        if (kc == 0 && o < p.O) p.db[(size_t)split * p.O + o] = bias;
+
+    float* dw = p.dw + split * p.stride;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j) {
+            const int n = n0 + wn + 32 * j + fc;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * fk;
+                if (m < p.O && n < p.I) dw[(size_t)m * p.I + n] = acc[i][j][e];
+            }
+        }
+    if (want_db) {  // (uniform; the last barrier above closed the buffers)
+        double* sum = reinterpret_cast<double*>(lds);
+#pragma unroll
+        for (int c = 0; c < AC; ++c) sum[a_kc * BM + a_cg * AC + c] = bias[c];
+        __syncthreads();
+        for (int m = tid; m < BM; m += NT)
+            if (m0 + m < p.O) p.db[split * p.stride + m0 + m] = (float)((sum[m] + sum[BM + m]) + (sum[2 * BM + m] + sum[3 * BM + m]));
     }
 }
 
-// out[i] = sum over splits, in order
-__global__ __launch_bounds__(256) void act8_sum_splits_kernel(const float* part, int S, size_t n, size_t stride, float* out) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-        float a = 0.f;
-        for (int s = 0; s < S; ++s) a += part[(size_t)s * stride + i];
-        out[i] = a;
+// Few outputs (up to 16 G): nothing to share between waves, and the codes are the whole traffic.  A wave owns 256 columns and a range of
+// rows and takes both operands from global memory straight into the MFMA's registers, no LDS: v_mfma_f32_16x16x32_bf16 wants rows
+// 8 (l / 16) .. + 7 of column l % 16 in lane l, and WHICH column of dw that is, is free: with the lane's 16 codes per row (one
+// load) being columns 16 (l % 16) + t, tile t = 0 .. 15 takes byte t of every load.
+template <typename T, int G>
+__global__ __launch_bounds__(256, 2) void act8_wgrad_narrow_kernel(const WgradP p) {
+    constexpr int N = Terms<T>::N;
+    __shared__ float lds[G * 16 * 256];
+    __shared__ double lds_db[4][G * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = lane & 15, k8 = lane >> 4;
+    const int tn = blockIdx.x % p.tiles_n, split = blockIdx.x / p.tiles_n;
+    const int n0 = tn * 256;
+    const size_t r_begin = (size_t)split * p.rows_per;
+    const size_t r_end = r_begin + p.rows_per < p.rows ? r_begin + p.rows_per : p.rows;
+    int col = n0 + 16 * c;
+    col = col < p.pitch ? col : p.pitch - 16;  // (columns that nobody stores)
+    f32x4 acc[G][16];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[g][t][e] = 0.f;
+    double bias[G];
+    int off[G];
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+        bias[g] = 0.0;
+        off[g] = 16 * g + c < p.O ? 16 * g + c : p.O - 1;
+    }
+    const T* dy = (const T*)p.dy;
+    for (size_t r0 = r_begin + 32 * wave; r0 < r_end; r0 += 128) {
+        u32x4_t q[8];
+        float s[8], a[G][8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const size_t r = r0 + 8 * k8 + j;
+            const bool in = r < r_end;
+            const size_t rr = in ? r : r_end - 1;
+            q[j] = *reinterpret_cast<const u32x4_any*>(p.codes + rr * p.pitch + col);
+            s[j] = act8_scale(p.exps[rr * p.groups + col / ACT8_GROUP]);
+#pragma unroll
+            for (int g = 0; g < G; ++g) a[g][j] = to_f32(dy[rr * p.lddy + off[g]]);
+            if (!in) {
+                s[j] = 0.f;
+#pragma unroll
+                for (int g = 0; g < G; ++g) a[g][j] = 0.f;
+            }
+        }
+        u32x4_t at[G][N];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            split_terms<N>(a[g], at[g]);
+            bias[g] += (double)(((a[g][0] + a[g][1]) + (a[g][2] + a[g][3])) + ((a[g][4] + a[g][5]) + (a[g][6] + a[g][7])));
+        }
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            u32x4_t b;
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+                b[h] = top_halves(code_value(q[2 * h + 1][t >> 2], t & 3, s[2 * h + 1], p.zero), code_value(q[2 * h][t >> 2], t & 3, s[2 * h], p.zero));
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    acc[g][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, at[g][k]), __builtin_bit_cast(bf16x8_t, b),
+                                                                        acc[g][t], 0, 0, 0);
+        }
+    }
+    // the four waves in order; lane l holds rows 4 (l / 16) + e of dw's tile and its column l % 16
+    for (int w = 0; w < 4; ++w) {
+        if (wave == w) {
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float* at = lds + (g * 16 + 4 * k8 + e) * 256 + 16 * t + c;
+                        *at = w ? *at + acc[g][t][e] : acc[g][t][e];
+                    }
+        }
+        __syncthreads();
+    }
+    float* dw = p.dw + split * p.stride;
+    const int rows_out = p.O < 16 * G ? p.O : 16 * G;
+    for (int i = threadIdx.x; i < rows_out * 256; i += 256) {
+        const int o = i >> 8, n = i & 255;  // column n: lane n / 16, tile n % 16
+        if (n0 + n < p.I) dw[(size_t)o * p.I + n0 + n] = lds[o * 256 + 16 * (n & 15) + (n >> 4)];
+    }
+    if (p.db && tn == 0) {
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            bias[g] += __shfl_xor(bias[g], 16, 64);
+            bias[g] += __shfl_xor(bias[g], 32, 64);
+            if (k8 == 0) lds_db[wave][16 * g + c] = bias[g];
+        }
+        __syncthreads();
+        if (threadIdx.x < rows_out)
+            p.db[split * p.stride + threadIdx.x] =
+                (float)((lds_db[0][threadIdx.x] + lds_db[1][threadIdx.x]) + (lds_db[2][threadIdx.x] + lds_db[3][threadIdx.x]));
     }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
+enum WgradKind { WGRAD_NARROW1, WGRAD_NARROW2, WGRAD_64, WGRAD_128, WGRAD_256 };
+constexpr int WGRAD_MOST = 1 << 24;
 struct WgradPlan {
+    WgradKind kind;
     int tiles_m, tiles_n, splits;
     size_t rows_per;
 };
 
+#ifdef SWEEP
+#include <stdlib.h>
+static int envi(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
+#define WANT_NARROW envi("WN", 1024)
+#define WANT_64 envi("W64", 1024)
+#define WANT_128 envi("W128", 512)
+#define MIN_ROWS envi("MINR", 128)
+#else
+#define WANT_NARROW 1024
+#define WANT_64 1024
+#define WANT_128 512
+#define MIN_ROWS 128
+#endif
 static WgradPlan wgrad_plan(size_t rows, int O, int I) {
     WgradPlan q;
-    q.tiles_m = ceil_div(O, 32);
-    q.tiles_n = ceil_div(I, 32);
+    int bm, bn, want;
+    if (O <= 32) {
+        q.kind = O <= 16 ? WGRAD_NARROW1 : WGRAD_NARROW2;
+        bm = 32;
+        bn = 256;
+        want = WANT_NARROW;
+    } else if (O >= 192 && I >= 192) {
+        q.kind = WGRAD_256;
+        bm = bn = 256;
+        want = 256;
+    } else if (O > 64 && I > 64) {
+        q.kind = WGRAD_128;
+        bm = bn = 128;
+        want = WANT_128;
+    } else {
+        q.kind = WGRAD_64;
+        bm = bn = 64;
+        want = WANT_64;
+    }
+    q.tiles_m = ceil_div(O, bm);
+    q.tiles_n = ceil_div(I, bn);
     const size_t tiles = (size_t)q.tiles_m * q.tiles_n;
-    size_t s = (4096 + tiles - 1) / tiles;
-    const size_t most = (rows + 127) / 128;
+    size_t s = want / tiles;
+    const size_t most = (rows + MIN_ROWS - 1) / MIN_ROWS;
     s = s < 1 ? 1 : s > most ? most : s;
-    if (s > 64) s = 64;
     q.rows_per = ((rows + s - 1) / s + 31) / 32 * 32;
     q.splits = (int)((rows + q.rows_per - 1) / q.rows_per);
     return q;
 }
 
 template <typename T>
-static void wgrad_launch(const WgradP& p, hipStream_t s) {
+static void wgrad_launch(WgradKind kind, const WgradP& p, hipStream_t s) {
     const unsigned grid = (unsigned)p.tiles_m * p.tiles_n * p.splits;
-    hipLaunchKernelGGL((act8_wgrad_simple_kernel<T>), dim3(grid), dim3(64), 0, s, p);
+    switch (kind) {
+        case WGRAD_NARROW1: hipLaunchKernelGGL((act8_wgrad_narrow_kernel<T, 1>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_NARROW2: hipLaunchKernelGGL((act8_wgrad_narrow_kernel<T, 2>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_64: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, 64, 64, 32, 32>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_128: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, 128, 128, 64, 64>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_256: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, 256, 256, 64, 128>), dim3(grid), dim3(512), 0, s, p); break;
+    }
 }
 
 static unsigned stream_grid(size_t vecs) {
@@ -219,7 +585,7 @@ extern "C" int dun_act8_pack(const void* x, int64_t ldx, uint8_t* codes, uint8_t
     DUN_REQUIRE(x && codes && exps, "dun_act8_pack: null tensor");
     DUN_REQUIRE(ldx >= cols, "dun_act8_pack: row stride %lld below %d columns", (long long)ldx, cols);
     DUN_REQUIRE(((uintptr_t)codes & 7) == 0, "dun_act8_pack: codes need 8-byte alignment");
-    const int groups = ceil_div(cols, ACT8_GROUP), E = dtype == DUN_F32 ? 4 : 8;
+    const int groups = ceil_div(cols, ACT8_GROUP);
     const u32 vpr = (u32)groups * (ACT8_GROUP / E);
     const size_t vecs = (size_t)rows * vpr;
     const dim3 grid(stream_grid(vecs));
@@ -242,7 +608,7 @@ extern "C" int dun_act8_unpack(const uint8_t* codes, const uint8_t* exps, void* 
     DUN_REQUIRE(out && codes && exps, "dun_act8_unpack: null tensor");
     DUN_REQUIRE(ldo >= cols, "dun_act8_unpack: row stride %lld below %d columns", (long long)ldo, cols);
     DUN_REQUIRE(((uintptr_t)codes & 7) == 0, "dun_act8_unpack: codes need 8-byte alignment");
-    const int groups = ceil_div(cols, ACT8_GROUP), E = dtype == DUN_F32 ? 4 : 8;
+    const int groups = ceil_div(cols, ACT8_GROUP);
     const u32 vpr = (u32)groups * (ACT8_GROUP / E);
     const size_t vecs = (size_t)rows * vpr;
     const dim3 grid(stream_grid(vecs));
@@ -275,14 +641,16 @@ extern "C" int dun_act8_weight_grad(const void* dy, int64_t lddy, const uint8_t*
     hipStream_t s = (hipStream_t)stream;
     const size_t n = (size_t)outs * cols;
     if (rows == 0) {  // (no splits to add up: zeros)
-        hipLaunchKernelGGL(act8_sum_splits_kernel, dim3(stream_grid(n)), dim3(256), 0, s, (const float*)nullptr, 0, n, n, dw);
-        if (db) hipLaunchKernelGGL(act8_sum_splits_kernel, dim3(stream_grid(outs)), dim3(256), 0, s, (const float*)nullptr, 0, (size_t)outs, (size_t)outs, db);
+        launch_zero_floats(dw, n, s);
+        if (db) launch_zero_floats(db, outs, s);
         DUN_LAUNCH_CHECK();
         return DUN_OK;
     }
     DUN_REQUIRE(dy && codes && exps, "dun_act8_weight_grad: null tensor");
     DUN_REQUIRE(lddy >= outs, "dun_act8_weight_grad: row stride %lld below %d columns", (long long)lddy, outs);
     DUN_REQUIRE(((uintptr_t)codes & 7) == 0, "dun_act8_weight_grad: codes need 8-byte alignment");
+    // (offsets inside 32 rows are 32-bit numbers in the kernels)
+    DUN_REQUIRE(lddy <= WGRAD_MOST && cols <= WGRAD_MOST, "dun_act8_weight_grad: row stride %lld or %d columns above %d", (long long)lddy, cols, WGRAD_MOST);
     const WgradPlan q = wgrad_plan((size_t)rows, outs, cols);
     DUN_REQUIRE((size_t)q.tiles_m * q.tiles_n * q.splits <= 0x7fffffffu, "dun_act8_weight_grad: %d x %d is too large a gradient", outs, cols);
     const size_t need = dun_act8_weight_grad_workspace_floats(rows, outs, cols, dtype);
@@ -292,8 +660,9 @@ extern "C" int dun_act8_weight_grad(const void* dy, int64_t lddy, const uint8_t*
     p.dy = dy;
     p.codes = codes;
     p.exps = exps;
+    p.stride = db ? n + outs : n;  // a split's dw and db lie one behind the other: one launch adds both up
     p.dw = need ? ws : dw;
-    p.db = !db ? nullptr : need ? ws + q.splits * n : db;
+    p.db = !db ? nullptr : need ? ws + n : db;
     p.lddy = (size_t)lddy;
     p.rows = (size_t)rows;
     p.rows_per = q.rows_per;
@@ -306,17 +675,14 @@ extern "C" int dun_act8_weight_grad(const void* dy, int64_t lddy, const uint8_t*
     p.splits = q.splits;
     p.zero = relu ? 0.f : 128.f;
     if (dtype == DUN_F32)
-        wgrad_launch<float>(p, s);
+        wgrad_launch<float>(q.kind, p, s);
     else if (dtype == DUN_BF16)
-        wgrad_launch<bf16_t>(p, s);
+        wgrad_launch<bf16_t>(q.kind, p, s);
     else
-        wgrad_launch<fp16_t>(p, s);
+        wgrad_launch<fp16_t>(q.kind, p, s);
     DUN_LAUNCH_CHECK();
     if (need) {
-        hipLaunchKernelGGL(act8_sum_splits_kernel, dim3(stream_grid(n)), dim3(256), 0, s, (const float*)ws, q.splits, n, n, dw);
-        if (db)
-            hipLaunchKernelGGL(act8_sum_splits_kernel, dim3(stream_grid(outs)), dim3(256), 0, s, (const float*)(ws + q.splits * n), q.splits,
-                               (size_t)outs, (size_t)outs, db);
+        launch_sum_rows(ws, q.splits, p.stride, dw, n, db, s);
         DUN_LAUNCH_CHECK();
     }
     return DUN_OK;

@@ -8,16 +8,15 @@
 //
 // Both directions move bytes: forward reads x (and res) once and writes y, backward reads x or its codes and dy and
 // writes dx.  So a row stays in the registers of the lanes that loaded it -- a TEAM of 8 to 64 lanes of a wave for rows of
-// up to 2048 elements, a workgroup for longer ones -- and the statistics are taken there in two passes over registers
-// (mean first, then squares of differences: no cancellation for rows far from zero), all in fp32.  Rows longer than what 1024
-// lanes hold are walked in memory.  The column sums dw, db, ds are kept per lane over all rows that a team visits (a lane always
+// up to 1024 elements, a workgroup for up to 8192 -- and the statistics are taken there in two passes over registers
+// (mean first, then squares of differences: no cancellation for rows far from zero), all in fp32.  Longer rows are walked in
+// memory.  The column sums dw, db, ds are kept per lane over all rows that a team visits (a lane always
 // sees the same columns), added up over a workgroup in LDS in a fixed order, and over workgroups by a second small
 // kernel: no atomics, the same bits every time.
 #include "rows.h"
 
 namespace dun {
 
-constexpr int LN_MAX_PER_LANE = 32;   // elements of a row that a lane holds
 constexpr int LN_LONG_THREADS = 1024;
 
 struct LnFwdP {
@@ -79,49 +78,61 @@ struct TeamSum {
     }
 };
 
-template <int TEAM> constexpr int ln_block() { return TEAM > 256 ? TEAM : 256; }
+struct Yes { static constexpr bool value = true; };
+struct No { static constexpr bool value = false; };
+
+template <int TEAM> constexpr int ln_block() { return TEAM > 64 ? TEAM : 256; }
+
+// Chunks of a lane that lie inside the row whatever its length, by the choice of the team (ln_team): the last chunk may end early, of
+// 256 x 4 the last two
+template <int TEAM, int CH> constexpr int ln_whole() { return TEAM == 256 && CH == 4 ? 2 : CH - 1; }
+
+template <typename T, int TEAM, int CH>
+__device__ __forceinline__ void ln_load_row(const T* row, int t, int cols, RawVec<T>* v) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        const int i0 = (c * TEAM + t) * E;
+        if (c < ln_whole<TEAM, CH>())
+            v[c].load(row, i0);
+        else
+            v[c].load_end(row, i0, cols);
+    }
+}
 
 template <typename T, int TEAM, int CH>
 __global__ __launch_bounds__(ln_block<TEAM>()) void ln_forward_kernel(const LnFwdP p) {
-    constexpr int E = Row<T>::E, TPB = ln_block<TEAM>() / TEAM;
+    constexpr int TPB = ln_block<TEAM>() / TEAM;
     __shared__ float red[TEAM > 64 ? 2 * (TEAM / 64) : 1];
     TeamSum<TEAM> sum(red);
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    const float n = (float)p.cols;
+    const float n = (float)p.cols, floor_ = p.relu ? 0.f : -INFINITY;
     for (size_t row = (size_t)blockIdx.x * TPB + team; row < p.rows; row += (size_t)gridDim.x * TPB) {
-        const T* x = (const T*)p.x + row * p.ldx;
-        float v[CH][E], r[CH][E];
-#pragma unroll
-        for (int c = 0; c < CH; ++c) load_part(x, (c * TEAM + t) * E, p.cols, v[c]);
+        RawVec<T> xv[CH], rv[CH];
+        ln_load_row<T, TEAM, CH>((const T*)p.x + row * p.ldx, t, p.cols, xv);
         if (p.res) {
-            const T* res = (const T*)p.res + row * p.ldr;
-#pragma unroll
-            for (int c = 0; c < CH; ++c) load_part(res, (c * TEAM + t) * E, p.cols, r[c]);
+            ln_load_row<T, TEAM, CH>((const T*)p.res + row * p.ldr, t, p.cols, rv);
         } else {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int e = 0; e < E; ++e) r[c][e] = 0.f;
+                for (int e = 0; e < RawVec<T>::W; ++e) rv[c].w[e] = 0;
         }
-        if (p.relu) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[c][e] = rectify(v[c][e]);
-        }
+        auto z = [&](int c, int e) { return max_nan(xv[c][e], floor_); };
         float s = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int e = 0; e < E; ++e) s += v[c][e];
+            for (int e = 0; e < E; ++e) s += z(c, e);
         const float mean = sum(s) / n;
         s = 0.f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) xv[c].forget();
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int i0 = (c * TEAM + t) * E;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const float d = i0 + e < p.cols ? v[c][e] - mean : 0.f;
+                const float d = c < ln_whole<TEAM, CH>() || i0 + e < p.cols ? z(c, e) - mean : 0.f;
                 s += d * d;
             }
         }
@@ -130,79 +141,94 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_forward_kernel(const LnFw
             p.mean[row] = mean;
             p.rstd[row] = rstd;
         }
-        if (p.xc) {
+        T* y = (T*)p.y + row * p.ldy;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) xv[c].forget();
+        // (the choices are the same for every row; made once here, not once per chunk)
+        auto finish = [&](auto affine, auto keep_x, auto keep_y) {
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int i0 = (c * TEAM + t) * E;
-                u32 w[E / 4];
-                const u32 byte = act8_pack<E>(v[c], p.relu, w);
-                if (i0 < p.groups * ACT8_GROUP) {
-                    act8_store_words<E>(p.xc + (row * p.groups) * ACT8_GROUP + i0, w);
-                    if (i0 % ACT8_GROUP == 0) p.xe[row * p.groups + i0 / ACT8_GROUP] = (uint8_t)byte;
+                constexpr bool any = !decltype(affine)::value;
+                RawVec<float> w, b;
+                if (!any || p.w) {
+                    if (c < ln_whole<TEAM, CH>()) w.load(p.w, i0); else w.load_end(p.w, i0, p.cols);
+                }
+                if (!any || p.b) {
+                    if (c < ln_whole<TEAM, CH>()) b.load(p.b, i0); else b.load_end(p.b, i0, p.cols);
+                }
+                if (keep_x.value && (!any || p.xc)) {
+                    float v[E];
+                    u32 byte;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) v[e] = z(c, e);
+                    const u32 word = act8_pack(v, p.relu, &byte);
+                    act8_store(p.xc, p.xe, row, p.groups, i0, word, byte);
+                }
+                float o[E];
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    float h = (z(c, e) - mean) * rstd;
+                    if (!any || p.w) h *= w[e];
+                    if (!any || p.b) h += b[e];
+                    o[e] = h + rv[c][e];
+                }
+                store_part(y, i0, p.cols, o);
+                if (keep_y.value && (!any || p.yc)) {
+                    // the checkpoint holds what the next layer reads: the output as it is stored
+                    u32 byte;
+#pragma unroll
+                    for (int e = 0; e < E; ++e) o[e] = i0 + e < p.cols ? to_f32(from_f32<T>(o[e])) : 0.f;
+                    const u32 word = act8_pack(o, false, &byte);
+                    act8_store(p.yc, p.ye, row, p.groups, i0, word, byte);
                 }
             }
-        }
-        T* y = (T*)p.y + row * p.ldy;
-#pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int i0 = (c * TEAM + t) * E;
-            float o[E], w[E], b[E];
-            if (p.w) load_f32<E>(p.w, i0, p.cols, w);
-            if (p.b) load_f32<E>(p.b, i0, p.cols, b);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                float h = (v[c][e] - mean) * rstd;
-                if (p.w) h *= w[e];
-                if (p.b) h += b[e];
-                o[e] = h + r[c][e];
-            }
-            store_part(y, i0, p.cols, o);
-            if (p.yc) {
-                // the checkpoint holds what the next layer reads: the output as it is stored
-                u32 q[E / 4];
-#pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = i0 + e < p.cols ? to_f32(from_f32<T>(o[e])) : 0.f;
-                const u32 byte = act8_pack<E>(o, false, q);
-                if (i0 < p.groups * ACT8_GROUP) {
-                    act8_store_words<E>(p.yc + (row * p.groups) * ACT8_GROUP + i0, q);
-                    if (i0 % ACT8_GROUP == 0) p.ye[row * p.groups + i0 / ACT8_GROUP] = (uint8_t)byte;
-                }
-            }
-        }
+        };
+        if (p.w && p.b && !p.xc && !p.yc)
+            finish(Yes(), No(), No());
+        else if (p.w && p.b && p.xc && !p.yc)
+            finish(Yes(), Yes(), No());
+        else
+            finish(No(), Yes(), Yes());
     }
 }
 
-// z of a lane's chunk in backward: the checkpoint's values, or x itself (rectified)
+// z of a lane's chunk in backward: x (rectified), or the checkpoint's word and its group's byte
+template <typename T>
+__device__ __forceinline__ void ln_fetch_codes(const LnBwdP& p, size_t row, int i0, RawVec<T>& raw) {
+    const int last = p.groups * ACT8_GROUP - E;
+    const int i = i0 < last ? i0 : last;
+    const u32 word = *reinterpret_cast<const u32*>(p.xc + row * p.groups * ACT8_GROUP + i);
+    const u32 byte = p.xe[row * p.groups + i / ACT8_GROUP];
+    // (past the row's groups: a code that stands for a number)
+    raw.w[0] = i0 <= last ? word : 0u;
+    raw.w[1] = i0 <= last ? byte : 0u;
+}
 template <typename T>
 __device__ __forceinline__ void ln_bwd_z(const LnBwdP& p, size_t row, int i0, float* v) {
-    constexpr int E = Row<T>::E;
+    RawVec<T> raw;
     if (p.xc) {
-        if (i0 < p.groups * ACT8_GROUP) {
-            u32 w[E / 4];
-            act8_load_words<E>(p.xc + (row * p.groups) * ACT8_GROUP + i0, w);
-            act8_values<E>(w, p.xe[row * p.groups + i0 / ACT8_GROUP], p.relu ? 0.f : 128.f, v);
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = 0.f;
-        }
+        ln_fetch_codes(p, row, i0, raw);
+        act8_values(raw.w[0], raw.w[1], p.relu ? 0.f : 128.f, v);
     } else {
-        load_part((const T*)p.x + row * p.ldx, i0, p.cols, v);
-        if (p.relu) {
+        const float floor_ = p.relu ? 0.f : -INFINITY;
+        raw.load_end((const T*)p.x + row * p.ldx, i0, p.cols);
 #pragma unroll
-            for (int e = 0; e < E; ++e) v[e] = rectify(v[e]);
-        }
+        for (int e = 0; e < E; ++e) v[e] = max_nan(raw[e], floor_);
     }
 }
 
-template <typename T, int TEAM, int CH, int K>
+// K: column sums wanted (0, 2 or 3).  MASK: rows may be rectified (p.relu), so z itself is kept for ReLU's mask and xhat is worked out a
+// second time, two operations per element against six for a mask of bits.
+template <typename T, int TEAM, int CH, int K, bool MASK>
 __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnBwdP p) {
-    constexpr int E = Row<T>::E, BLOCK = ln_block<TEAM>(), TPB = BLOCK / TEAM;
+    constexpr int BLOCK = ln_block<TEAM>(), TPB = BLOCK / TEAM;
     constexpr int SPAN = TEAM * E * CH;  // columns that a team covers
     __shared__ float red[TEAM > 64 ? 2 * (TEAM / 64) : 1];
     __shared__ float acc_lds[TEAM > 64 ? 1 : (K > 0 ? K : 1) * SPAN];
     TeamSum<TEAM> sum(red);
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    const float n = (float)p.cols;
+    const float n = (float)p.cols, floor_ = MASK && p.relu ? 0.f : -INFINITY;
     float acc[K > 0 ? K : 1][CH][E];
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -211,40 +237,54 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnB
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[k][c][e] = 0.f;
     for (size_t row = (size_t)blockIdx.x * TPB + team; row < p.rows; row += (size_t)gridDim.x * TPB) {
-        const T* dy = (const T*)p.dy + row * p.lddy;
+        RawVec<T> dv[CH], zv[CH];
         float h[CH][E], g[CH][E];
+        ln_load_row<T, TEAM, CH>((const T*)p.dy + row * p.lddy, t, p.cols, dv);
+        if (p.xc) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) load_part(dy, (c * TEAM + t) * E, p.cols, g[c]);
-#pragma unroll
-        for (int c = 0; c < CH; ++c) ln_bwd_z<T>(p, row, (c * TEAM + t) * E, h[c]);
+            for (int c = 0; c < CH; ++c) ln_fetch_codes(p, row, (c * TEAM + t) * E, zv[c]);
+        } else {
+            ln_load_row<T, TEAM, CH>((const T*)p.x + row * p.ldx, t, p.cols, zv);
+        }
         const float mean = p.mean[row], rstd = p.rstd[row];
-        u32 live = ~0u;  // bit c * E + e: z > 0, or NaN (CH * E <= 32)
-        if (p.relu) {
-            live = 0;
+        if (p.xc) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) act8_values(zv[c].w[0], zv[c].w[1], p.relu ? 0.f : 128.f, h[c]);
+        } else {
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
-                for (int e = 0; e < E; ++e) live |= (u32)!(h[c][e] <= 0.f) << (c * E + e);
+                for (int e = 0; e < E; ++e) h[c][e] = MASK ? max_nan(zv[c][e], floor_) : zv[c][e];
         }
         float s1 = 0.f, s2 = 0.f;
+        auto first = [&](auto weighted) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int i0 = (c * TEAM + t) * E;
-            float w[E];
-            if (p.w) load_f32<E>(p.w, i0, p.cols, w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                // (columns past the row's end hold dy = 0: they add nothing to any sum, whatever h is there, as long as it is finite)
-                h[c][e] = (h[c][e] - mean) * rstd;
-                if (K > 0) {
-                    acc[0][c][e] += g[c][e] * h[c][e];
-                    acc[1][c][e] += g[c][e];
+            for (int c = 0; c < CH; ++c) {
+                const int i0 = (c * TEAM + t) * E;
+                RawVec<float> w;
+                if (weighted.value) {
+                    if (c < ln_whole<TEAM, CH>()) w.load(p.w, i0); else w.load_end(p.w, i0, p.cols);
                 }
-                if (p.w) g[c][e] *= w[e];
-                s1 += g[c][e];
-                s2 += g[c][e] * h[c][e];
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    // (columns past the row's end hold dy = 0: they add nothing to any sum)
+                    const float xhat = (h[c][e] - mean) * rstd;
+                    if (!MASK) h[c][e] = xhat;
+                    const float d = dv[c][e];
+                    if (K > 0) {
+                        acc[0][c][e] += d * xhat;
+                        acc[1][c][e] += d;
+                    }
+                    g[c][e] = weighted.value ? d * w[e] : d;
+                    s1 += g[c][e];
+                    s2 += g[c][e] * xhat;
+                }
             }
-        }
+        };
+        if (p.w)
+            first(Yes());
+        else
+            first(No());
         s1 = sum(s1) / n;
         s2 = sum(s2) / n;
         T* dx = (T*)p.dx + row * p.lddx;
@@ -254,9 +294,10 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnB
             float o[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                o[e] = rstd * (g[c][e] - s1 - h[c][e] * s2);
-                if (!((live >> (c * E + e)) & 1u)) o[e] = 0.f;
-                if (K > 2) acc[K > 2 ? 2 : 0][c][e] += i0 + e < p.cols ? o[e] : 0.f;
+                const float xhat = MASK ? (h[c][e] - mean) * rstd : h[c][e];
+                o[e] = rstd * (g[c][e] - s1 - xhat * s2);
+                if (MASK) o[e] = h[c][e] <= floor_ ? 0.f : o[e];
+                if (K > 2) acc[K > 2 ? 2 : 0][c][e] += c < ln_whole<TEAM, CH>() || i0 + e < p.cols ? o[e] : 0.f;
             }
             store_part(dx, i0, p.cols, o);
         }
@@ -306,7 +347,7 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnB
 // ---- rows longer than 1024 lanes hold: the same sums, the row read again instead of kept ------------------------------------
 template <typename T>
 __global__ __launch_bounds__(LN_LONG_THREADS) void ln_forward_long_kernel(const LnFwdP p) {
-    constexpr int E = Row<T>::E, STEP = LN_LONG_THREADS * E;
+    constexpr int STEP = LN_LONG_THREADS * E;
     __shared__ float red[2 * (LN_LONG_THREADS / 64)];
     TeamSum<LN_LONG_THREADS> sum(red);
     const float n = (float)p.cols;
@@ -341,8 +382,8 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_forward_long_kernel(const 
             float r[E], w[E], b[E], o[E];
             load_part(x, i0, p.cols, v);
             if (res) load_part(res, i0, p.cols, r);
-            if (p.w) load_f32<E>(p.w, i0, p.cols, w);
-            if (p.b) load_f32<E>(p.b, i0, p.cols, b);
+            if (p.w) load_part(p.w, i0, p.cols, w);
+            if (p.b) load_part(p.b, i0, p.cols, b);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 if (p.relu) v[e] = rectify(v[e]);
@@ -352,19 +393,17 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_forward_long_kernel(const 
                 o[e] = res ? h + r[e] : h;
             }
             if (p.xc) {
-                u32 q[E / 4];
-                const u32 byte = act8_pack<E>(v, p.relu, q);
-                act8_store_words<E>(p.xc + (row * p.groups) * ACT8_GROUP + i0, q);
-                if (i0 % ACT8_GROUP == 0) p.xe[row * p.groups + i0 / ACT8_GROUP] = (uint8_t)byte;
+                u32 byte;
+                const u32 word = act8_pack(v, p.relu, &byte);
+                act8_store(p.xc, p.xe, row, p.groups, i0, word, byte);
             }
             store_part(y, i0, p.cols, o);
             if (p.yc) {
-                u32 q[E / 4];
+                u32 byte;
 #pragma unroll
                 for (int e = 0; e < E; ++e) o[e] = i0 + e < p.cols ? to_f32(from_f32<T>(o[e])) : 0.f;
-                const u32 byte = act8_pack<E>(o, false, q);
-                act8_store_words<E>(p.yc + (row * p.groups) * ACT8_GROUP + i0, q);
-                if (i0 % ACT8_GROUP == 0) p.ye[row * p.groups + i0 / ACT8_GROUP] = (uint8_t)byte;
+                const u32 word = act8_pack(o, false, &byte);
+                act8_store(p.yc, p.ye, row, p.groups, i0, word, byte);
             }
         }
     }
@@ -372,7 +411,7 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_forward_long_kernel(const 
 
 template <typename T>
 __global__ __launch_bounds__(LN_LONG_THREADS) void ln_backward_long_kernel(const LnBwdP p) {
-    constexpr int E = Row<T>::E, STEP = LN_LONG_THREADS * E;
+    constexpr int STEP = LN_LONG_THREADS * E;
     __shared__ float red[2 * (LN_LONG_THREADS / 64)];
     TeamSum<LN_LONG_THREADS> sum(red);
     const float n = (float)p.cols;
@@ -387,7 +426,7 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_backward_long_kernel(const
         for (int i0 = t0; i0 < p.cols; i0 += STEP) {
             load_part(dy, i0, p.cols, g);
             ln_bwd_z<T>(p, row, i0, h);
-            if (p.w) load_f32<E>(p.w, i0, p.cols, w);
+            if (p.w) load_part(p.w, i0, p.cols, w);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const float q = p.w ? g[e] * w[e] : g[e];
@@ -401,7 +440,7 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_backward_long_kernel(const
             float o[E];
             load_part(dy, i0, p.cols, g);
             ln_bwd_z<T>(p, row, i0, h);
-            if (p.w) load_f32<E>(p.w, i0, p.cols, w);
+            if (p.w) load_part(p.w, i0, p.cols, w);
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const bool dead = p.relu && h[e] <= 0.f;
@@ -420,119 +459,78 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_backward_long_kernel(const
     }
 }
 
-// out[i] = sum over the workgroups' partial rows: 32 columns x 8 slices of the rows per workgroup, slices added in order
-__global__ __launch_bounds__(256) void ln_reduce_kernel(const float* part, size_t P, size_t n, float* out) {
-    __shared__ float lds[8][32];
-    const int c = threadIdx.x & 31, s = threadIdx.x >> 5;
-    const size_t i = (size_t)blockIdx.x * 32 + c;
-    float a = 0.f;
-    if (i < n) {
-        size_t r = s;
-        float a1 = 0.f, a2 = 0.f, a3 = 0.f;
-        for (; r + 24 < P; r += 32) {
-            a += part[r * n + i];
-            a1 += part[(r + 8) * n + i];
-            a2 += part[(r + 16) * n + i];
-            a3 += part[(r + 24) * n + i];
-        }
-        for (; r < P; r += 8) a += part[r * n + i];
-        a = (a + a1) + (a2 + a3);
-    }
-    lds[s][c] = a;
-    __syncthreads();
-    if (s == 0 && i < n) {
-#pragma unroll
-        for (int j = 1; j < 8; ++j) a += lds[j][c];
-        out[i] = a;
-    }
-}
-
-__global__ __launch_bounds__(256) void ln_zero_kernel(float* p, size_t n) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0.f;
-}
-
 // ---- host side ---------------------------------------------------------------------------------------------------------------
-// The team for rows of `cols` elements: the fewest lanes that hold a row at 16 bytes each up to a wave, then more vectors per
-// lane up to 32 elements, then more lanes.  0: too long for registers.
-static int ln_team(int cols, int E, int* ch) {
+// Teams and vectors of four elements per lane, by the elements that a team holds: the fewest lanes up to a wave, then more vectors per
+// lane, then more waves.  What decides is the bytes in flight: few registers per row for many rows at a time, but no idle lanes.
+// 65536 x 2048 fp32, forward / backward: 64 x 8 237 / 330 us, 256 x 2 200 / 297 us (a plain copy of as many bytes: 208 / 312);
+// 16391 x 1031 bf16: 256 x 2, half of its lanes idle, 34 / 60 us, 128 x 3 27 / 43 us.
+#define DUN_LN_TEAMS(X) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(64, 2) X(64, 3) X(64, 4) X(128, 3) X(256, 2) X(256, 4) X(1024, 2)
+
+static int ln_team(int cols, int* ch) {
     const int vecs = ceil_div(cols, E);
-    *ch = 1;
-    for (int team = 8; team <= 64; team *= 2)
-        if (vecs <= team) return team;
-    const int most = LN_MAX_PER_LANE / E;
-    for (int team = 64; team <= 1024; team *= 4)
-        for (int c = 2; c <= most; c *= 2)
-            if (vecs <= team * c && (team == 64 || c == most)) {
-                *ch = c;
-                return team;
-            }
-    return 0;
+#define DUN_LN_PICK(TEAM, CH) \
+    if (vecs <= TEAM * CH) {  \
+        *ch = CH;             \
+        return TEAM;          \
+    }
+    DUN_LN_TEAMS(DUN_LN_PICK)
+#undef DUN_LN_PICK
+    *ch = 0;
+    return 0;  // too long for registers
 }
 
-// Workgroups of a backward pass: enough to fill 256 CUs at the registers that the row takes, no more than there are rows
-static size_t ln_backward_blocks(size_t rows, int cols, int E) {
+// Workgroups of a backward pass, each with a partial row of sums: what 256 CUs hold at once, no more than there are rows (65536 x 2048
+// fp32 from the checkpoint: 768 243 us, 1024 231 us, 1536 278 us)
+static size_t ln_backward_blocks(size_t rows, int cols) {
     int ch;
-    const int team = ln_team(cols, E, &ch);
+    const int team = ln_team(cols, &ch);
     if (team == 0) return rows < 256 ? rows : 256;
-    const size_t tpb = team < 256 ? 256 / team : 1;
-    const size_t need = (rows + tpb - 1) / tpb, most = ch == 1 ? 1024 : 512;
-    return need < most ? need : most;
+    const size_t tpb = team <= 64 ? 256 / team : 1;
+    const size_t need = (rows + tpb - 1) / tpb;
+    return need < 1024 ? need : 1024;
 }
 
 template <typename T>
 static void ln_launch_forward(const LnFwdP& p, hipStream_t s) {
     int ch;
-    const int team = ln_team(p.cols, Row<T>::E, &ch);
-    const size_t tpb = team && team < 256 ? 256 / team : 1;
+    const int team = ln_team(p.cols, &ch);
+    const size_t tpb = team && team <= 64 ? 256 / team : 1;
     const size_t need = (p.rows + tpb - 1) / tpb;
-    const dim3 grid((unsigned)(need < (1u << 20) ? need : (1u << 20)));
+        const dim3 grid((unsigned)(need < (1u << 20) ? need : (1u << 20)));
 #define DUN_LN_FWD(TEAM, CH)                                                                               \
     if (team == TEAM && ch == CH) {                                                                        \
         hipLaunchKernelGGL((ln_forward_kernel<T, TEAM, CH>), grid, dim3(ln_block<TEAM>()), 0, s, p);       \
         return;                                                                                            \
     }
-    constexpr int M = LN_MAX_PER_LANE / Row<T>::E;
-    DUN_LN_FWD(8, 1)
-    DUN_LN_FWD(16, 1)
-    DUN_LN_FWD(32, 1)
-    DUN_LN_FWD(64, 1)
-    DUN_LN_FWD(64, 2)
-    DUN_LN_FWD(64, 4)
-    if constexpr (M == 8) DUN_LN_FWD(64, M)
-    DUN_LN_FWD(256, M)
-    DUN_LN_FWD(1024, M)
+    DUN_LN_TEAMS(DUN_LN_FWD)
     hipLaunchKernelGGL((ln_forward_long_kernel<T>), dim3((unsigned)(p.rows < 65536 ? p.rows : 65536)), dim3(LN_LONG_THREADS), 0, s, p);
 #undef DUN_LN_FWD
 }
 
-template <typename T, int K>
+template <typename T, int K, bool MASK>
 static void ln_launch_backward_k(const LnBwdP& p, unsigned blocks, hipStream_t s) {
     int ch;
-    const int team = ln_team(p.cols, Row<T>::E, &ch);
-#define DUN_LN_BWD(TEAM, CH)                                                                               \
-    if (team == TEAM && ch == CH) {                                                                        \
-        hipLaunchKernelGGL((ln_backward_kernel<T, TEAM, CH, K>), dim3(blocks), dim3(ln_block<TEAM>()), 0, s, p); \
-        return;                                                                                            \
+    const int team = ln_team(p.cols, &ch);
+#define DUN_LN_BWD(TEAM, CH)                                                                                     \
+    if (team == TEAM && ch == CH) {                                                                              \
+        hipLaunchKernelGGL((ln_backward_kernel<T, TEAM, CH, K, MASK>), dim3(blocks), dim3(ln_block<TEAM>()), 0, s, p); \
+        return;                                                                                                  \
     }
-    constexpr int M = LN_MAX_PER_LANE / Row<T>::E;
-    DUN_LN_BWD(8, 1)
-    DUN_LN_BWD(16, 1)
-    DUN_LN_BWD(32, 1)
-    DUN_LN_BWD(64, 1)
-    DUN_LN_BWD(64, 2)
-    DUN_LN_BWD(64, 4)
-    if constexpr (M == 8) DUN_LN_BWD(64, M)
-    DUN_LN_BWD(256, M)
-    DUN_LN_BWD(1024, M)
-    hipLaunchKernelGGL((ln_backward_long_kernel<T>), dim3(blocks), dim3(LN_LONG_THREADS), 0, s, p);
+    DUN_LN_TEAMS(DUN_LN_BWD)
 #undef DUN_LN_BWD
+    hipLaunchKernelGGL((ln_backward_long_kernel<T>), dim3(blocks), dim3(LN_LONG_THREADS), 0, s, p);
 }
 
 template <typename T>
 static void ln_launch_backward(const LnBwdP& p, unsigned blocks, hipStream_t s) {
-    if (p.K == 0) return ln_launch_backward_k<T, 0>(p, blocks, s);
-    if (p.K == 2) return ln_launch_backward_k<T, 2>(p, blocks, s);
-    ln_launch_backward_k<T, 3>(p, blocks, s);
+    if (p.K == 0)
+        ln_launch_backward_k<T, 0, true>(p, blocks, s);
+    else if (p.K == 3)
+        ln_launch_backward_k<T, 3, true>(p, blocks, s);
+    else if (p.relu)
+        ln_launch_backward_k<T, 2, true>(p, blocks, s);
+    else
+        ln_launch_backward_k<T, 2, false>(p, blocks, s);
 }
 
 }  // namespace dun
@@ -541,7 +539,7 @@ using namespace dun;
 
 extern "C" size_t dun_layer_norm_backward_workspace_floats(int64_t rows, int cols, int dtype, int sums) {
     if (rows <= 0 || cols <= 0 || sums < 2) return 0;
-    const size_t blocks = ln_backward_blocks((size_t)rows, cols, dtype == DUN_F32 ? 4 : 8);
+    const size_t blocks = ln_backward_blocks((size_t)rows, cols);
     return blocks > 1 ? blocks * (size_t)sums * cols : 0;
 }
 
@@ -601,8 +599,7 @@ extern "C" int dun_layer_norm_backward(const void* dy, int64_t lddy, const void*
     hipStream_t s = (hipStream_t)stream;
     if (rows == 0) {
         if (sums) {
-            const size_t n = (size_t)sums * cols;
-            hipLaunchKernelGGL(ln_zero_kernel, dim3((unsigned)(n < (1u << 18) ? (n + 255) / 256 : 1024)), dim3(256), 0, s, sums_out, n);
+            launch_zero_floats(sums_out, (size_t)sums * cols, s);
             DUN_LAUNCH_CHECK();
         }
         return DUN_OK;
@@ -611,7 +608,7 @@ extern "C" int dun_layer_norm_backward(const void* dy, int64_t lddy, const void*
     DUN_REQUIRE(!x != !x_codes && !x_codes == !x_exps, "dun_layer_norm_backward: either x or its codes and exponents");
     DUN_REQUIRE(((uintptr_t)x_codes & 7) == 0, "dun_layer_norm_backward: codes need 8-byte alignment");
     DUN_REQUIRE(lddy >= cols && lddx >= cols && (!x || ldx >= cols), "dun_layer_norm_backward: a row stride is below %d columns", cols);
-    const size_t blocks = ln_backward_blocks((size_t)rows, cols, dtype == DUN_F32 ? 4 : 8);
+    const size_t blocks = ln_backward_blocks((size_t)rows, cols);
     const size_t need = dun_layer_norm_backward_workspace_floats(rows, cols, dtype, sums);
     DUN_REQUIRE(need == 0 || (ws && ws_floats >= need), "dun_layer_norm_backward: workspace of %zu floats, %zu needed", ws_floats, need);
     LnBwdP p;
@@ -642,7 +639,7 @@ extern "C" int dun_layer_norm_backward(const void* dy, int64_t lddy, const void*
     DUN_LAUNCH_CHECK();
     if (need) {
         const size_t n = (size_t)sums * cols;
-        hipLaunchKernelGGL(ln_reduce_kernel, dim3((unsigned)((n + 31) / 32)), dim3(256), 0, s, ws, blocks, n, sums_out);
+        launch_sum_rows(ws, blocks, n, sums_out, n, nullptr, s);
         DUN_LAUNCH_CHECK();
     }
     return DUN_OK;

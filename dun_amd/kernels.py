@@ -444,6 +444,8 @@ class HipBackend(object):
         with L.on_device(dy):
             dy, ld = L.rows_view(dy)
             rows, outs = dy.shape
+            if ld > 1 << 24:  # (the kernels' row stride ends there)
+                dy, ld = dy.contiguous(), outs
             dt = L.ROW_DTYPES[dy.dtype]
             f = dict(device=dy.device, dtype=torch.float32)
             if dw is None:

@@ -469,7 +469,7 @@ int dun_act8_unpack(const uint8_t* codes, const uint8_t* exps, void* out, int64_
  * A value has at most 8 significant bits and a power-of-two scale, hence is a bf16 number; dy is taken apart into bf16
  * numbers (fp32: three, fp16: two, bf16: one) whose sum it is; the products are exact and accumulate in fp32 on the bf16 matrix
  * cores.  (Parts of dy below 2^-133 are lost.  A non-finite dy gives a non-finite, not necessarily the same, result.)
- * ws: scratch of dun_act8_weight_grad_workspace_floats() floats. */
+ * cols and lddy are at most 2^24.  ws: scratch of dun_act8_weight_grad_workspace_floats() floats. */
 size_t dun_act8_weight_grad_workspace_floats(int64_t rows, int outs, int cols, int dtype);
 int dun_act8_weight_grad(const void* dy, int64_t lddy, const uint8_t* codes, const uint8_t* exps, float* dw, float* db,
                          float* ws, size_t ws_floats, int64_t rows, int outs, int cols, int dtype, int relu,

@@ -102,7 +102,7 @@ def test_c_entries_refuse_without_launching():
         assert lib.dun_act8_unpack(*[a[n] for n in "c e x ld rows cols dt relu s".split()]) == bad, k
     base = dict(dy=p, ld=6, c=p, e=p, dw=p, db=None, ws=None, nws=0, rows=4, outs=6, cols=8, dt=0, relu=0, s=None)
     for k in (dict(dy=None), dict(c=None), dict(e=None), dict(dw=None), dict(ld=5), dict(outs=0), dict(cols=0), dict(rows=-1), dict(dt=5),
-              dict(c=p + 1), dict(rows=1 << 20)):
+              dict(c=p + 1), dict(rows=1 << 20), dict(ld=(1 << 24) + 1), dict(cols=(1 << 24) + 1)):
         assert lib.dun_act8_weight_grad(*[dict(base, **k)[n] for n in base]) == bad, k
         assert b"dun_act8_weight_grad" in lib.dun_last_error()
 
