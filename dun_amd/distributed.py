@@ -86,8 +86,9 @@ def shard(net, group=None, sync_bn=True, overlap=True, grad_bucket_blocks=2):
         tensors = [p.data for p in net.model.parameters() if getattr(p, "_dun_flat_owner", None) is None]
         tensors += [b for b in net.model.buffers() if getattr(net.model, "flat_params", None) is None]
         if getattr(net.model, "flat_params", None) is not None:
-            tensors += [net.model.flat_params, net.model.running_mean, net.model.running_var,
-                        net.model.num_batches_tracked]
+            # (a trunk without BatchNorm has no running statistics)
+            tensors += [t for t in (net.model.flat_params, net.model.running_mean, net.model.running_var,
+                                    net.model.num_batches_tracked) if t is not None]
         tensors += [p.data for p in net.prob_model.parameters()]
         tensors += [p.data for p in net.f_neg_loglike.parameters()]
         if spec.world > 1:

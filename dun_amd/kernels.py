@@ -139,6 +139,58 @@ class FcBuffers(object):
         return bool(L.lib().dun_fc_head_is_fused(C.byref(self.c)))
 
 
+class LnFcBuffers(object):
+    """Device buffers of one LayerNorm trunk at a fixed (batch, depth, mode).
+
+    Training keeps what backward reads: every block's input and rectified Linear output, in float32 (``act_bits`` 32) or as
+    8-bit checkpoints (8: 1 + 1/32 bytes an element, and one float32 hidden state that is updated in place); prediction
+    keeps nothing."""
+
+    def __init__(self, model, B, depth, train):
+        dev = model.flat_params.device
+        W, O = model.width, model.output_dim
+        f = dict(device=dev, dtype=torch.float32)
+        self.B, self.depth, self.train = B, depth, train
+        self.keep32 = train and model.act_bits == 32
+        self.keep8 = train and model.act_bits == 8
+        planes = depth + 1 if self.keep32 else 1
+        self.H = torch.empty(planes, B, W, **f)
+        self.Z = torch.empty(max(planes - 1, 1), B, W, **f)
+        self.stats = torch.empty(max(depth, 1), 2, B, **f) if train else None
+        self.Hq = self.Zq = None
+        if self.keep8:
+            self.Hq = backend().act8_buffers((depth + 1) * B, W, dev)
+            self.Zq = backend().act8_buffers(max(depth, 1) * B, W, dev)
+        self._act_shape = (depth + 1, B, O)
+        self.act = None  # a fresh [depth+1,B,O] tensor per forward: callers may keep what they get
+        self.x = None
+        self.generation = 0  # bumped by every forward that writes these buffers
+        self.G = self.dU = self.Wt = self.sums = None
+
+    def new_act(self):
+        self.act = torch.empty(self._act_shape, device=self.H.device, dtype=torch.float32)
+
+    def h(self, i):
+        return self.H[i if self.keep32 else 0]
+
+    def z(self, i):
+        return self.Z[i if self.keep32 else 0]
+
+    def rows8(self, packed, i):
+        """Checkpoint of plane i."""
+        return None if packed is None else (packed[0][i * self.B:(i + 1) * self.B], packed[1][i * self.B:(i + 1) * self.B])
+
+    def ensure_backward(self, model):
+        if self.G is None:
+            W, dev = model.width, self.H.device
+            f = dict(device=dev, dtype=torch.float32)
+            self.G, self.dU = torch.empty(self.B, W, **f), torch.empty(self.B, W, **f)
+            self.Wt = torch.empty(model.n_layers, W, W, **f)   # both operands of dU W along the reduction
+            self.sums = torch.empty(max(model.n_layers, 1), 3, W, **f)
+            self.ones = torch.ones(self.B, 1, **f)
+            self.splitk = torch.empty(2 * W * max(W, model.input_dim), **f)
+
+
 class HipBackend(object):
     name = "hip"
 
@@ -297,6 +349,9 @@ class HipBackend(object):
     def fc_buffers(self, model, B, depth, train):
         return FcBuffers(model, B, depth, train)
 
+    def ln_fc_buffers(self, model, B, depth, train):
+        return LnFcBuffers(model, B, depth, train)
+
     def _fc(self, name, buf, *args):
         fn = getattr(L.lib(), name)
         L.check(fn(C.byref(buf.c), *args, L.stream_ptr(buf.H.device)), name)
@@ -344,10 +399,10 @@ class HipBackend(object):
         self._fc("dun_fc_bwd_end", buf)
 
     # ---- shared head over all exits -------------------------------------------------------------------
-    def head_forward(self, H, w, b):
+    def head_forward(self, H, w, b, out=None):
         rows, K = H.shape[0], H.shape[1]
         O = w.shape[0]
-        act = torch.empty(rows, O, device=H.device, dtype=torch.float32)
+        act = torch.empty(rows, O, device=H.device, dtype=torch.float32) if out is None else out
         L.check(L.lib().dun_head_forward(L.f32(H), L.f32(w), L.f32(b), rows, K, O, L.f32(act), L.stream_ptr(H.device)),
                 "dun_head_forward")
         return act
@@ -460,8 +515,9 @@ class HipBackend(object):
         return dw, db
 
     def layer_norm_forward(self, x, w, b, eps, res=None, relu=False, want_stats=True, pack_x=False, pack_y=False, out=None,
-                           x_packed=None, y_packed=None):
-        """-> (y, stats [2, rows] or None, packed z or None, packed y or None); w, b: float32 [cols] or None."""
+                           stats=None, x_packed=None, y_packed=None):
+        """-> (y, stats [2, rows] or None, packed z or None, packed y or None); w, b: float32 [cols] or None.  `out` may be
+        `res`."""
         with L.on_device(x):
             x, ldx = L.rows_view(x)
             rows, cols = x.shape
@@ -470,7 +526,8 @@ class HipBackend(object):
             if res is not None:
                 res, ldr = L.rows_view(res)
             y = torch.empty(rows, cols, device=dev, dtype=x.dtype) if out is None else out
-            stats = torch.empty(2, rows, device=dev, dtype=torch.float32) if want_stats else None
+            if want_stats and stats is None:
+                stats = torch.empty(2, rows, device=dev, dtype=torch.float32)
             xq = (self.act8_buffers(rows, cols, dev) if x_packed is None else x_packed) if pack_x else None
             yq = (self.act8_buffers(rows, cols, dev) if y_packed is None else y_packed) if pack_y else None
             L.check(L.lib().dun_layer_norm_forward(

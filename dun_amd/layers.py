@@ -28,3 +28,14 @@ class bern_MLPBlock_nores(nn.Module):
 
     def forward(self, x, b):
         return self.block(x)
+
+
+class bern_LNBlock(nn.Module):
+    """x + b * LayerNorm(ReLU(Linear(x))); no counterpart in the reference, whose blocks normalise over the batch"""
+
+    def __init__(self, width):
+        super(bern_LNBlock, self).__init__()
+        self.block = nn.Sequential(nn.Linear(width, width), nn.ReLU(), nn.LayerNorm(width))
+
+    def forward(self, x, b):
+        return x + b * self.block(x)

@@ -10,7 +10,7 @@ import torch
 import torch.nn as nn
 
 from . import kernels
-from .layers import bern_MLPBlock, bern_MLPBlock_nores
+from .layers import bern_LNBlock, bern_MLPBlock, bern_MLPBlock_nores
 
 _SEG_ALIGN = 64  # floats: every segment of the flat buffers starts on a 256-byte boundary
 _KINDS = ("w_in", "b_in", "w_out", "b_out", "w", "b", "gamma", "beta")
@@ -116,18 +116,7 @@ class arq_uncert_fc_resnet(nn.Module):
                 p._dun_flat_owner = self
                 self._param_list.append(p)
                 self._grad_views.append(gdst)
-            L, W = self.n_layers, self.width
-            rm = torch.zeros(L, W, device=dev)
-            rv = torch.ones(L, W, device=dev)
-            nbt = torch.zeros(L, device=dev, dtype=torch.int64)
-            for i, blk in enumerate(self.stochstic_layers):
-                bn = blk.block[2]
-                rm[i].copy_(bn.running_mean)
-                rv[i].copy_(bn.running_var)
-                nbt[i] = bn.num_batches_tracked
-                bn.running_mean = rm[i]
-                bn.running_var = rv[i]
-                bn.num_batches_tracked = nbt[i]
+            rm, rv, nbt = self._flatten_norm(dev)
         self.flat_params, self.flat_grads = flat, gflat
         # captured steps hold the addresses of the buffers they were captured on: a rebuilt flat buffer (load_state_dict,
         # .to()) may land on the old parameter address while its gradient buffer does not, so the wrappers key their
@@ -137,6 +126,22 @@ class arq_uncert_fc_resnet(nn.Module):
         self._fc_cache = {}
         # every parameter of the module tree lives in the flat buffer (what the whole-step hipGraph relies on)
         self._all_params_flat = all(getattr(q, "_dun_flat_owner", None) is self for q in self.parameters())
+
+    def _flatten_norm(self, dev):
+        """BatchNorm's buffers of all blocks as rows of three tensors."""
+        L, W = self.n_layers, self.width
+        rm = torch.zeros(L, W, device=dev)
+        rv = torch.ones(L, W, device=dev)
+        nbt = torch.zeros(L, device=dev, dtype=torch.int64)
+        for i, blk in enumerate(self.stochstic_layers):
+            bn = blk.block[2]
+            rm[i].copy_(bn.running_mean)
+            rv[i].copy_(bn.running_var)
+            nbt[i] = bn.num_batches_tracked
+            bn.running_mean = rm[i]
+            bn.running_var = rv[i]
+            bn.num_batches_tracked = nbt[i]
+        return rm, rv, nbt
 
     def _apply(self, fn, *args, **kwargs):
         super(arq_uncert_fc_resnet, self)._apply(fn, *args, **kwargs)
@@ -214,9 +219,12 @@ class arq_uncert_fc_resnet(nn.Module):
             if len(self._fc_cache) >= 4:  # keep the cache bounded: training + a few inference shapes
                 for k in [k for k in self._fc_cache if not k[2]][:1] or list(self._fc_cache)[:1]:
                     del self._fc_cache[k]
-            buf = kernels.backend().fc_buffers(self, B, depth, train)
+            buf = self._make_buffers(B, depth, train)
             self._fc_cache[key] = buf
         return buf
+
+    def _make_buffers(self, B, depth, train):
+        return kernels.backend().fc_buffers(self, B, depth, train)
 
     supports_head_objective = True  # forward(x, objective=HeadObjective): likelihood pass inside the head kernels
 
@@ -329,3 +337,103 @@ class arq_uncert_fc_resnet(nn.Module):
 class arq_uncert_fc_MLP(arq_uncert_fc_resnet):
     residual = False
     _block_cls = bern_MLPBlock_nores
+
+
+class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
+    """The residual trunk with LayerNorm in its blocks, h + LayerNorm(ReLU(Linear(h))): no counterpart in the reference,
+    whose blocks normalise over the batch (src/DUN/layers.py:33-42).
+
+    Rows do not couple: a batch of one row trains, prediction and training compute the same function, and a sharded job
+    exchanges gradients and likelihood sums only.  ``act_bits=8`` keeps what the backward reads as 8-bit checkpoints
+    (dun_amd.act8), a quarter of the memory: a block's LayerNorm then runs its backward from the checkpoint of the
+    rectified Linear output, its Linear's and the head's weight gradients from the checkpoints of the hidden states.
+    Same wrappers, flat parameters, optimiser and checkpoints as the BatchNorm trunk.  Weights in float32."""
+    _block_cls = bern_LNBlock
+    supports_head_objective = False
+
+    def __init__(self, input_dim, output_dim, width, n_layers, w_prior=None, BMA_prior=False, act_bits=32):
+        if act_bits not in (8, 32):
+            raise ValueError("act_bits is 32 or 8 (got %r)" % (act_bits,))
+        super(arq_uncert_fc_resnet_ln, self).__init__(input_dim, output_dim, width, n_layers, w_prior, BMA_prior)
+        self.act_bits, self.ln_eps = act_bits, 1e-5
+
+    def _flatten_norm(self, dev):
+        return None, None, None
+
+    def _make_buffers(self, B, depth, train):
+        return kernels.backend().ln_fc_buffers(self, B, depth, train)
+
+    def _run_forward(self, x, depth, train, objective=None):
+        if x.dim() != 2 or x.shape[1] != self.input_dim:
+            raise RuntimeError("expected x of shape [B, %d], got %s" % (self.input_dim, tuple(x.shape)))
+        if x.shape[0] == 0:
+            raise RuntimeError("an empty batch has nothing to train on")
+        be = kernels.backend()
+        B, W, O, din = x.shape[0], self.width, self.output_dim, self.input_dim
+        x = x.detach().to(torch.float32).contiguous()
+        buf = self._get_buffers(B, depth, train)
+        buf.generation += 1
+        buf.new_act()
+        buf.x = x
+        p = self.stacked
+        be.gemm(x, p["w_in"], B, W, din, bias=p["b_in"], out=buf.h(0))
+        if buf.keep8:
+            be.act8_pack(buf.h(0), False, out=buf.rows8(buf.Hq, 0))
+        if not buf.keep32:
+            be.head_forward(buf.h(0), p["w_out"], p["b_out"], out=buf.act[0])
+        for i in range(depth):
+            h, z = buf.h(i), buf.z(i)
+            be.gemm(h, p["w"][i], B, W, W, bias=p["b"][i], relu=True, out=z)
+            be.layer_norm_forward(z, p["gamma"][i], p["beta"][i], self.ln_eps, res=h, relu=True, want_stats=train,
+                                  stats=buf.stats[i] if train else None, out=buf.h(i + 1), pack_x=buf.keep8, pack_y=buf.keep8,
+                                  x_packed=buf.rows8(buf.Zq, i), y_packed=buf.rows8(buf.Hq, i + 1))
+            if not buf.keep32:
+                be.head_forward(buf.h(i + 1), p["w_out"], p["b_out"], out=buf.act[i + 1])
+        if buf.keep32:  # every hidden state is there: the shared head over all depths at once
+            be.head_forward(buf.H.view((depth + 1) * B, W), p["w_out"], p["b_out"], out=buf.act.view((depth + 1) * B, O))
+        return buf
+
+    def _run_backward(self, buf, dact):
+        be = kernels.backend()
+        buf.ensure_backward(self)
+        B, W, O, din, depth = buf.B, self.width, self.output_dim, self.input_dim, buf.depth
+        p, g, dist = self.stacked, self.stacked_grad, self._dist
+        dact = dact.detach().to(torch.float32).contiguous()
+        rows = dact.view((depth + 1) * B, O)
+        if buf.keep8:
+            be.act8_weight_grad(rows, buf.Hq, W, False, dw=g["w_out"], db=g["b_out"])
+        else:
+            dw, db, _ = be.head_backward(buf.H.view((depth + 1) * B, W), p["w_out"], rows, need_dH=False)
+            g["w_out"].copy_(dw)
+            g["b_out"].copy_(db)
+        be.gemm(dact[depth], p["w_out"], B, W, O, b_kcontig=False, out=buf.G)
+        buf.Wt.copy_(p["w"].transpose(1, 2))
+        for k in ("w", "b", "gamma", "beta"):  # blocks past a truncated forward
+            if depth < self.n_layers:
+                g[k][depth:].zero_()
+        sent_from = self.n_layers
+        for i in range(depth - 1, -1, -1):
+            be.layer_norm_backward(buf.G, None if buf.keep8 else buf.z(i), buf.rows8(buf.Zq, i), p["gamma"][i], buf.stats[i],
+                                   relu=True, sums=3, dx=buf.dU, sums_out=buf.sums[i])
+            if buf.keep8:
+                be.act8_weight_grad(buf.dU, buf.rows8(buf.Hq, i), W, False, want_bias=False, dw=g["w"][i])
+            else:
+                be.gemm(buf.dU, buf.h(i), W, W, B, a_kcontig=False, b_kcontig=False, splitk_ws=buf.splitk, out=g["w"][i])
+            if dist is not None and (sent_from - i >= dist.grad_bucket_blocks or i == 0):
+                dist.reduce_gradient_async(g["w"][i:sent_from])
+                sent_from = i
+            be.gemm(buf.dU, buf.Wt[i], B, W, W, R=buf.G, U=dact[i], V=p["w_out"], out=buf.G)
+        if depth:
+            g["gamma"][:depth].copy_(buf.sums[:depth, 0])
+            g["beta"][:depth].copy_(buf.sums[:depth, 1])
+            g["b"][:depth].copy_(buf.sums[:depth, 2])
+        be.gemm(buf.G, buf.x, W, din, B, a_kcontig=False, b_kcontig=False, splitk_ws=buf.splitk, out=g["w_in"])
+        # (sum_b G: the head's weight gradient of a gradient of ones)
+        g["b_in"].copy_(be.head_backward(buf.G, p["w_out"][:1], buf.ones, need_dH=False)[0].view(W))
+        if dist is not None:
+            if depth == 0 and self.n_layers:
+                dist.reduce_gradient_async(g["w"])
+            dist.reduce_gradient_async(self.flat_grads, exclude=g["w"])
+        for q, gv in zip(self._param_list, self._grad_views):
+            if q.grad is not gv:
+                q.grad = gv

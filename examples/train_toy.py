@@ -10,7 +10,8 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 from dun_amd.datasets import Datafeed, load_agw_1d, load_matern_1d, load_my_1d, load_wiggle  # noqa: E402
 from dun_amd.probability import depth_categorical_VI  # noqa: E402
-from dun_amd.stochastic_fc_models import arq_uncert_fc_MLP, arq_uncert_fc_resnet  # noqa: E402
+from dun_amd.stochastic_fc_models import (arq_uncert_fc_MLP, arq_uncert_fc_resnet,  # noqa: E402
+                                          arq_uncert_fc_resnet_ln)
 from dun_amd.train_fc import train_fc_DUN  # noqa: E402
 from dun_amd.training_wrappers import DUN_VI  # noqa: E402
 
@@ -21,7 +22,10 @@ ap.add_argument('--N_layers', type=int, default=10)
 ap.add_argument('--width', type=int, default=100)
 ap.add_argument('--lr', type=float, default=1e-3)
 ap.add_argument('--wd', type=float, default=1e-4)
-ap.add_argument('--network', default='ResNet', choices=['ResNet', 'MLP'])
+ap.add_argument('--network', default='ResNet', choices=['ResNet', 'MLP', 'ResNetLN'],
+                help="ResNetLN: LayerNorm blocks instead of the reference's BatchNorm ones")
+ap.add_argument('--act_bits', type=int, default=32, choices=[32, 8],
+                help='ResNetLN: bits of the activations kept for the backward pass')
 ap.add_argument('--savedir', default='./saves/')
 ap.add_argument('--dataset', default='wiggle', choices=['wiggle', 'agw_1d', 'matern_1d', 'my_1d'],
                 help="the reference's --dataset values that need no download (train_toy.py:69-83)")
@@ -41,8 +45,9 @@ else:
 ds = Datafeed(torch.Tensor(X), torch.Tensor(Y))
 train = torch.utils.data.DataLoader(ds, batch_size=2048, shuffle=True)
 val = torch.utils.data.DataLoader(ds, batch_size=2048, shuffle=False)
-ctor = arq_uncert_fc_resnet if args.network == 'ResNet' else arq_uncert_fc_MLP
-model = ctor(X.shape[1], Y.shape[1], args.width, args.N_layers, w_prior=None, BMA_prior=False)
+ctor = {'ResNet': arq_uncert_fc_resnet, 'MLP': arq_uncert_fc_MLP, 'ResNetLN': arq_uncert_fc_resnet_ln}[args.network]
+kw = dict(act_bits=args.act_bits) if args.network == 'ResNetLN' else {}
+model = ctor(X.shape[1], Y.shape[1], args.width, args.N_layers, w_prior=None, BMA_prior=False, **kw)
 D = args.N_layers + 1
 net = DUN_VI(model, depth_categorical_VI([1 / D] * D, cuda=True), X.shape[0], lr=args.lr, momentum=0.9, cuda=True,
              schedule=None, regression=True, pred_sig=None, weight_decay=args.wd)

@@ -2,7 +2,7 @@
 import torch
 
 U32 = 2.0 ** -24  # half a step of float32, relative
-HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+HALF = {torch.float64: 2.0 ** -53, torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
 GROUP = 32
 
 
