@@ -16,8 +16,7 @@ namespace dun {
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef u32 u32x4_any __attribute__((ext_vector_type(4), aligned(8)));
-typedef u32 u32_any __attribute__((aligned(2)));
-typedef float f32x2_any __attribute__((ext_vector_type(2), aligned(4)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // ---- pack / unpack: elementwise streams -----------------------------------------------------------------------------------------
 // One vector of E columns per lane; a row is G * 32 / E vectors (padded groups included), so the lanes of a group are neighbours.
@@ -81,7 +80,6 @@ struct WgradP {
     size_t rows_per;  // rows of one split, a multiple of 32
     int O, I, groups, pitch;
     int tiles_m, tiles_n, splits;
-    float zero;
 };
 
 template <typename T> struct Terms { static constexpr int N = 1; };
@@ -110,27 +108,30 @@ __device__ __forceinline__ void split_terms(const float* x, u32x4_t* out) {
         }
     }
 }
-// (code - zero first: zero * scale overflows where a group's largest magnitude is 2^127 or more)
-__device__ __forceinline__ float code_value(u32 word, int j, float s, float zero) {
-    return ((float)((word >> (8 * j)) & 0xffu) - zero) * s;
+// value of byte j of a word of codes: unsigned, or signed (stored + 128; `word` has been turned into signed bytes by code_word)
+template <bool SIGNED>
+__device__ __forceinline__ u32 code_word(u32 word) { return SIGNED ? word ^ 0x80808080u : word; }
+template <bool SIGNED>
+__device__ __forceinline__ float code_value(u32 word, int j, float s) {
+    return SIGNED ? (float)(signed char)(word >> (8 * j)) * s : (float)((word >> (8 * j)) & 0xffu) * s;
 }
 
-// What a thread holds of dy between its load and the matrix cores: AC neighbouring columns of 8 rows
+// What a thread holds of dy between its load and the matrix cores: AC neighbouring columns of 8 rows.  `up`: the pair was loaded one column
+// early, because it passed the last one; its first column is the second that was loaded.
 template <typename T, int AC> struct DyRegs {
-    float v[8][AC];
-    __device__ __forceinline__ void get(int j, const float* p) {
-        if constexpr (AC == 2) {
-            const f32x2_any q = *reinterpret_cast<const f32x2_any*>(p);
-            v[j][0] = q[0];
-            v[j][1] = q[1];
-        } else {
-            v[j][0] = *p;
-        }
+    f32x2_t v[8];
+    __device__ __forceinline__ void get(int j, __amdgpu_buffer_rsrc_t r, u32 lane, u32 row) {
+        if constexpr (AC == 2)
+            v[j] = __builtin_bit_cast(f32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, lane, row, 0));
+        else
+            v[j][0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, lane, row, 0));
     }
-    __device__ __forceinline__ void get1(int j, int c, const float* p) { v[j][c] = *p; }
-    __device__ __forceinline__ void clear(int j) {
+    __device__ __forceinline__ void keep(int j, bool yes) { v[j] = yes ? v[j] : f32x2_t{0.f, 0.f}; }
+    __device__ __forceinline__ void align(bool up) {
+        if constexpr (AC == 2) {
 #pragma unroll
-        for (int c = 0; c < AC; ++c) v[j][c] = 0.f;
+            for (int j = 0; j < 8; ++j) v[j][0] = up ? v[j][1] : v[j][0];
+        }
     }
     __device__ __forceinline__ float value(int j, int c) const { return v[j][c]; }
     __device__ __forceinline__ void terms(int c, u32x4_t* out) const {
@@ -142,17 +143,20 @@ template <typename T, int AC> struct DyRegs {
 };
 template <typename T, int AC> struct DyRegs16 {
     u32 v[8];  // AC = 2: both columns in a word
-    __device__ __forceinline__ void get(int j, const T* p) {
+    __device__ __forceinline__ void get(int j, __amdgpu_buffer_rsrc_t r, u32 lane, u32 row) {
+        if constexpr (AC == 2)
+            v[j] = __builtin_amdgcn_raw_buffer_load_b32(r, lane, row, 0);
+        else
+            v[j] = (u16)__builtin_amdgcn_raw_buffer_load_b16(r, lane, row, 0);
+    }
+    __device__ __forceinline__ void keep(int j, bool yes) { v[j] = yes ? v[j] : 0u; }
+    __device__ __forceinline__ void align(bool up) {
         if constexpr (AC == 2) {
-            v[j] = *reinterpret_cast<const u32_any*>(p);
-        } else {
-            v[j] = p->bits;
+            const int by = up ? 16 : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] >>= by;
         }
     }
-    __device__ __forceinline__ void get1(int j, int c, const T* p) {
-        v[j] = c == 0 ? (u32)p->bits : (v[j] & 0xffffu) | ((u32)p->bits << 16);
-    }
-    __device__ __forceinline__ void clear(int j) { v[j] = 0; }
     __device__ __forceinline__ float value(int j, int c) const { return to_f32(T{(u16)(v[j] >> (16 * c))}); }
 };
 template <int AC> struct DyRegs<bf16_t, AC> : DyRegs16<bf16_t, AC> {
@@ -178,6 +182,11 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// A buffer of `bytes` from p on (0x00027000: raw 32-bit data)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* p, u32 bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000);
+}
+
 // A workgroup owns a BM x BN tile of dw over one range of rows and walks it 32 rows at a time through two LDS buffers of
 // bf16 operands: [column][32 rows], 64 bytes a column, N such planes for dy and one for the values.  While the matrix
 // cores work on one buffer, the rows two steps ahead are on their way into registers and those one step ahead are taken
@@ -186,11 +195,11 @@ __device__ __forceinline__ void lds_barrier() {
 // A column's four 16-byte chunks (8 rows each) and the column's place among its neighbours are permuted by its
 // index so that the writes (columns 1, 2 or 4 apart, one chunk) and the reads (columns in a row, one chunk) spread over the banks.
 __device__ __forceinline__ int lds_chunk(int col, int kc) {
-    const int a = (col >> 2) & 3;
-    return ((col & ~3) | ((col & 3) ^ a)) * 4 + (kc ^ a ^ ((col >> 4) & 3));
+    const int g = col >> 2;
+    return ((col & ~3) | ((col ^ g) & 3)) * 4 + (kc ^ (-g & 3) ^ ((g >> 2) & 3));
 }
 
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, bool SIGNED, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) >= 8 ? 2 : 1) void act8_wgrad_tile_kernel(const WgradP p) {
     constexpr int N = Terms<T>::N, NT = (BM / WM) * (BN / WN) * 64;
     constexpr int AC = 4 * BM / NT, BC = 8 * BN / NT;
@@ -215,83 +224,83 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) >
     const int steps = (int)((r_end - r_begin + 31) / 32);
 
     const int tid = threadIdx.x;
-    // dy: 8 rows x AC columns.  Columns past the last are read from the last: they make rows of dw that nobody stores.
+    // Loads: 8 rows x AC columns of dy, 4 rows x BC columns of codes (one group).  No branches around them and nothing done with what
+    // they bring before it is staged, or they would be waited for where they are issued.  Columns past the last are read from inside
+    // the row: they make rows or columns of dw that nobody stores.  The last step of a range takes the range's last 32 rows, and counts
+    // the ones it has seen before as zeros.  Through buffer descriptors that start at the step's first row: an offset of the lane
+    // that never changes plus one of the row.
     const int a_cg = tid % (BM / AC), a_kc = tid / (BM / AC);
-    const bool m_full = m0 + BM <= p.O;
-    // (addresses: a base that is the same for all lanes, plus a 32-bit offset of the lane that never changes)
-    u32 a_off[AC];
-#pragma unroll
-    for (int c = 0; c < AC; ++c) {
-        const int o = m0 + a_cg * AC + c;
-        a_off[c] = (u32)(a_kc * 8 * (u32)p.lddy + (o < p.O ? o : p.O - 1)) * (u32)sizeof(T);
-    }
-    const char* a_base = (const char*)p.dy + r_begin * p.lddy * sizeof(T);
+    const int a_col = m0 + a_cg * AC, a_most = p.O - AC;  // (O > 32 here)
+    const bool up = a_col > a_most;
     const u32 a_row = (u32)p.lddy * (u32)sizeof(T);
-    // codes: 4 rows x BC columns, one group
-    const int b_cg = tid % (BN / BC), b_kq = tid / (BN / BC);
+    const u32 a_off = (u32)a_kc * 8 * a_row + (u32)(up ? a_most : a_col) * (u32)sizeof(T);
+    // (neighbouring lanes take the two halves of a chunk: 32 lanes write all of 256 bytes)
+    const int b_cg = (tid >> 1) % (BN / BC), b_kq = (tid & 1) + 2 * (tid / (2 * BN / BC));
     int b_col = n0 + b_cg * BC;
     b_col = b_col < p.pitch ? b_col : p.pitch - BC;
     const u32 b_off = (u32)(b_kq * 4) * (u32)p.pitch + (u32)b_col;
     const u32 e_off = (u32)(b_kq * 4) * (u32)p.groups + (u32)(b_col / ACT8_GROUP);
-    const uint8_t* b_base = p.codes + r_begin * p.pitch;
-    const uint8_t* e_base = p.exps + r_begin * p.groups;
 
     DyRegs<T, AC> ra;
-    u32 rb[4], re[4];
-    auto get_a = [&](int j, int c) { return (const T*)(a_base + (size_t)j * a_row + a_off[c]); };
-    auto get_b = [&](int j) {
-        const uint8_t* q = b_base + (size_t)j * p.pitch + b_off;
-        return BC == 4 ? *reinterpret_cast<const u32*>(q) : (u32)*reinterpret_cast<const u16*>(q);
-    };
-    auto get_e = [&](int j) { return (u32)*(e_base + (size_t)j * p.groups + e_off); };
+    u32 rb[4][(BC + 3) / 4], re[4];
+    const int rest = (int)(r_end - r_begin) - 32 * (steps - 1);  // rows of the last step
+    const bool few = r_end < 32;                                 // (no 32 rows to take: only step 0 of all there is)
     auto load = [&](int step) {
-        const size_t left = r_end - r_begin - (size_t)step * 32;
-        if (left >= 32) {
+        const size_t r = step + 1 < steps ? r_begin + (size_t)step * 32 : r_end - 32;
+        const __amdgpu_buffer_rsrc_t da = rows_buffer((const char*)p.dy + r * a_row, 31 * a_row + (u32)p.O * (u32)sizeof(T));
+        const __amdgpu_buffer_rsrc_t db = rows_buffer(p.codes + r * p.pitch, 32 * (u32)p.pitch);
+        const __amdgpu_buffer_rsrc_t de = rows_buffer(p.exps + r * p.groups, 32 * (u32)p.groups);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                rb[j] = get_b(j);
-                re[j] = get_e(j);
-            }
-            if (m_full) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) ra.get(j, get_a(j, 0));
+        for (int j = 0; j < 4; ++j) {
+            const u32 at = (u32)j * (u32)p.pitch;
+            if constexpr (BC == 2) {
+                rb[j][0] = (u16)__builtin_amdgcn_raw_buffer_load_b16(db, b_off, at, 0);
+            } else if constexpr (BC == 4) {
+                rb[j][0] = __builtin_amdgcn_raw_buffer_load_b32(db, b_off, at, 0);
             } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int c = 0; c < AC; ++c) ra.get1(j, c, get_a(j, c));
+                const u32x2_t q = __builtin_amdgcn_raw_buffer_load_b64(db, b_off, at, 0);
+                rb[j][0] = q[0];
+                rb[j][(BC + 3) / 4 - 1] = q[1];
             }
-        } else {  // rows past the last are zeros in both operands (a value there could be a NaN)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                ra.clear(j);
-                if ((size_t)(a_kc * 8 + j) < left) {
-#pragma unroll
-                    for (int c = 0; c < AC; ++c) ra.get1(j, c, get_a(j, c));
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                rb[j] = p.zero != 0.f ? 0x80808080u : 0u;
-                re[j] = 0;
-                if ((size_t)(b_kq * 4 + j) < left) {
-                    rb[j] = get_b(j);
-                    re[j] = get_e(j);
-                }
-            }
+            re[j] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(de, e_off, (u32)j * (u32)p.groups, 0);
         }
-        a_base += (size_t)32 * a_row;
-        b_base += (size_t)32 * p.pitch;
-        e_base += (size_t)32 * p.groups;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ra.get(j, da, a_off, (u32)j * a_row);
+    };
+    auto load_few = [&] {  // rows past the last are read from the last, and count as zeros
+        const int last = (int)r_end - 1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = b_kq * 4 + j < last ? b_kq * 4 + j : last;
+#pragma unroll
+            for (int k = 0; k < (BC + 3) / 4; ++k) {
+                const uint8_t* q = p.codes + (size_t)r * p.pitch + b_col + 4 * k;
+                rb[j][k] = BC == 2 ? (u32)*reinterpret_cast<const u16*>(q) : *reinterpret_cast<const u32*>(q);
+            }
+            re[j] = p.exps[(size_t)r * p.groups + b_col / ACT8_GROUP];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = a_kc * 8 + j < last ? a_kc * 8 + j : last;
+            ra.get(j, rows_buffer(p.dy, (u32)last * a_row + (u32)p.O * (u32)sizeof(T)), a_off - (u32)a_kc * 8 * a_row + (u32)r * a_row, 0);
+        }
     };
 
     const bool want_db = p.db && tn == 0;
     double bias[AC];
 #pragma unroll
     for (int c = 0; c < AC; ++c) bias[c] = 0.0;
-    auto stage = [&](int buf) {
+    auto stage = [&](int buf, int step) {
+        if (step + 1 == steps && (rest < 32)) {  // (the same for the whole workgroup) zeros in both operands: a value there could be a NaN
+            const int lo = few ? 0 : 32 - rest, hi = few ? rest : 32;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) ra.keep(j, a_kc * 8 + j >= lo && a_kc * 8 + j < hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) re[j] = b_kq * 4 + j >= lo && b_kq * 4 + j < hi ? re[j] : 0u;
+        }
         u32x4_t* A = lds + buf * BUF;
         u32x4_t* B = A + N * PLANE_A;
+        if (m0 + BM > p.O) ra.align(up);  // (the same for the whole workgroup)
 #pragma unroll
         for (int c = 0; c < AC; ++c) {
             u32x4_t t[N];
@@ -310,12 +319,16 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) >
         }
         float s[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = act8_scale(re[j]);
+        for (int j = 0; j < 4; ++j) {
+            s[j] = act8_scale(re[j]);
+#pragma unroll
+            for (int k = 0; k < (BC + 3) / 4; ++k) rb[j][k] = code_word<SIGNED>(rb[j][k]);
+        }
 #pragma unroll
         for (int c = 0; c < BC; ++c) {
             u32x2_t w;
-            w[0] = top_halves(code_value(rb[1], c, s[1], p.zero), code_value(rb[0], c, s[0], p.zero));
-            w[1] = top_halves(code_value(rb[3], c, s[3], p.zero), code_value(rb[2], c, s[2], p.zero));
+            w[0] = top_halves(code_value<SIGNED>(rb[1][c / 4], c % 4, s[1]), code_value<SIGNED>(rb[0][c / 4], c % 4, s[0]));
+            w[1] = top_halves(code_value<SIGNED>(rb[3][c / 4], c % 4, s[3]), code_value<SIGNED>(rb[2][c / 4], c % 4, s[2]));
             reinterpret_cast<u32x2_t*>(B)[lds_chunk(b_cg * BC + c, b_kq >> 1) * 2 + (b_kq & 1)] = w;
         }
     };
@@ -330,50 +343,63 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) >
         for (int j = 0; j < CT; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    // A wave alone has to keep the matrix pipe busy for as long as its partner stages: the operands of the next 32 rows of dw are read
+    // from LDS before the products of these are issued.
     auto compute = [&](int buf) {
         const u32x4_t* A = lds + buf * BUF;
         const u32x4_t* B = A + N * PLANE_A;
+        u32x4_t a[2][N], b[2][CT];
+        auto read_a = [&](int g) {
+            const int at = lds_chunk(wm + 32 * (g % MT) + fc, 2 * (g / MT) + fk);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            u32x4_t b[CT];
+            for (int t = 0; t < N; ++t) a[g & 1][t] = A[t * PLANE_A + at];
+        };
+        auto read_b = [&](int ks) {
 #pragma unroll
-            for (int j = 0; j < CT; ++j) b[j] = B[lds_chunk(wn + 32 * j + fc, 2 * ks + fk)];
+            for (int j = 0; j < CT; ++j) b[ks][j] = B[lds_chunk(wn + 32 * j + fc, 2 * ks + fk)];
+        };
+        read_b(0);
+        read_a(0);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int at = lds_chunk(wm + 32 * i + fc, 2 * ks + fk);
-                u32x4_t a[N];
-#pragma unroll
-                for (int t = 0; t < N; ++t) a[t] = A[t * PLANE_A + at];
-#pragma unroll
-                for (int t = 0; t < N; ++t)
-#pragma unroll
-                    for (int j = 0; j < CT; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[t]), __builtin_bit_cast(bf16x8_t, b[j]),
-                                                                            acc[i][j], 0, 0, 0);
+        for (int g = 0; g < 2 * MT; ++g) {
+            if (g + 1 < 2 * MT) {
+                if ((g + 1) % MT == 0) read_b(1);
+                read_a(g + 1);
             }
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int t = 0; t < N; ++t)
+#pragma unroll
+                for (int j = 0; j < CT; ++j)
+                    acc[g % MT][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a[g & 1][t]), __builtin_bit_cast(bf16x8_t, b[g / MT][j]),
+                                                                             acc[g % MT][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
     // Two waves share a SIMD in the large tile: one of each pair takes its rows apart before its matrix products, the other after them, so
-    // that the vector and the matrix pipe both have work all the time.
-    const bool early = NT >= 512 && wave < NT / 128;
-    load(0);
-    stage(0);
+    // that the vector and the matrix pipe both have work all the time.  Between two barriers the early waves stage step k + 1 and
+    // multiply step k, the late ones multiply k and stage k + 1; with the loop turned by half a step for the late ones both do it in
+    // the same place of the code: stage, [late: barrier], multiply, [early: barrier].
+    const bool early = NT < 512 || wave < NT / 128;
+    if (few)
+        load_few();
+    else
+        load(0);
+    stage(0, 0);
     if (steps > 1) load(1);
     lds_barrier();
     for (int k = 0; k < steps; ++k) {
-        const bool more = k + 1 < steps;
-        if (early && more) {
-            stage((k + 1) & 1);
-            if (k + 2 < steps) load(k + 2);
+        const int s = early ? k + 1 : k;
+        if (s >= 1 && s < steps) {
+            stage(s & 1, s);
+            load(s + 1 < steps ? s + 1 : s);
         }
+        if (!early && k >= 1) lds_barrier();
         compute(k & 1);
-        if (!early && more) {
-            stage((k + 1) & 1);
-            if (k + 2 < steps) load(k + 2);
-        }
-        lds_barrier();
+        if (early) lds_barrier();
     }
+    if (!early) lds_barrier();
 
     float* dw = p.dw + split * p.stride;
 #pragma unroll
@@ -401,7 +427,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) >
 // rows and takes both operands from global memory straight into the MFMA's registers, no LDS: v_mfma_f32_16x16x32_bf16 wants rows
 // 8 (l / 16) .. + 7 of column l % 16 in lane l, and WHICH column of dw that is, is free: with the lane's 16 codes per row (one
 // load) being columns 16 (l % 16) + t, tile t = 0 .. 15 takes byte t of every load.
-template <typename T, int G>
+template <typename T, bool SIGNED, int G>
 __global__ __launch_bounds__(256, 2) void act8_wgrad_narrow_kernel(const WgradP p) {
     constexpr int N = Terms<T>::N;
     __shared__ float lds[G * 16 * 256];
@@ -429,24 +455,37 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_narrow_kernel(const WgradP 
         off[g] = 16 * g + c < p.O ? 16 * g + c : p.O - 1;
     }
     const T* dy = (const T*)p.dy;
-    for (size_t r0 = r_begin + 32 * wave; r0 < r_end; r0 += 128) {
+    // the next 32 rows are on their way while these are worked on (two groups of outputs leave no registers for that)
+    constexpr bool AHEAD = G == 1;
+    u32x4_t qn[8];
+    u32 en[8];
+    T an[G][8];
+    auto fetch = [&](size_t r0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const size_t r = r0 + 8 * k8 + j, rr = r < r_end ? r : r_end - 1;
+            qn[j] = *reinterpret_cast<const u32x4_any*>(p.codes + rr * p.pitch + col);
+            en[j] = p.exps[rr * p.groups + col / ACT8_GROUP];
+#pragma unroll
+            for (int g = 0; g < G; ++g) an[g][j] = dy[rr * p.lddy + off[g]];
+        }
+    };
+    size_t r0 = r_begin + 32 * wave;
+    if (AHEAD && r0 < r_end) fetch(r0);
+    for (; r0 < r_end; r0 += 128) {
+        if (!AHEAD) fetch(r0);
         u32x4_t q[8];
         float s[8], a[G][8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const size_t r = r0 + 8 * k8 + j;
-            const bool in = r < r_end;
-            const size_t rr = in ? r : r_end - 1;
-            q[j] = *reinterpret_cast<const u32x4_any*>(p.codes + rr * p.pitch + col);
-            s[j] = act8_scale(p.exps[rr * p.groups + col / ACT8_GROUP]);
+            const bool in = r0 + 8 * k8 + j < r_end;  // rows past the last are zeros in both operands
 #pragma unroll
-            for (int g = 0; g < G; ++g) a[g][j] = to_f32(dy[rr * p.lddy + off[g]]);
-            if (!in) {
-                s[j] = 0.f;
+            for (int k = 0; k < 4; ++k) q[j][k] = code_word<SIGNED>(qn[j][k]);
+            s[j] = in ? act8_scale(en[j]) : 0.f;
 #pragma unroll
-                for (int g = 0; g < G; ++g) a[g][j] = 0.f;
-            }
+            for (int g = 0; g < G; ++g) a[g][j] = in ? to_f32(an[g][j]) : 0.f;
         }
+        if (AHEAD && r0 + 128 < r_end) fetch(r0 + 128);
         u32x4_t at[G][N];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
@@ -458,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_narrow_kernel(const WgradP 
             u32x4_t b;
 #pragma unroll
             for (int h = 0; h < 4; ++h)
-                b[h] = top_halves(code_value(q[2 * h + 1][t >> 2], t & 3, s[2 * h + 1], p.zero), code_value(q[2 * h][t >> 2], t & 3, s[2 * h], p.zero));
+                b[h] = top_halves(code_value<SIGNED>(q[2 * h + 1][t >> 2], t & 3, s[2 * h + 1]), code_value<SIGNED>(q[2 * h][t >> 2], t & 3, s[2 * h]));
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -503,7 +542,7 @@ __global__ __launch_bounds__(256, 2) void act8_wgrad_narrow_kernel(const WgradP 
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------------
-enum WgradKind { WGRAD_NARROW1, WGRAD_NARROW2, WGRAD_64, WGRAD_128, WGRAD_256 };
+enum WgradKind { WGRAD_64, WGRAD_64x256, WGRAD_128, WGRAD_256, WGRAD_NARROW1, WGRAD_NARROW2 };
 constexpr int WGRAD_MOST = 1 << 24;
 struct WgradPlan {
     WgradKind kind;
@@ -511,61 +550,82 @@ struct WgradPlan {
     size_t rows_per;
 };
 
-#ifdef SWEEP
-#include <stdlib.h>
-static int envi(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
-#define WANT_NARROW envi("WN", 1024)
-#define WANT_64 envi("W64", 1024)
-#define WANT_128 envi("W128", 512)
-#define MIN_ROWS envi("MINR", 128)
-#else
-#define WANT_NARROW 1024
-#define WANT_64 1024
-#define WANT_128 512
-#define MIN_ROWS 128
-#endif
+// `s` ranges of whole 32-row steps, of at least 64 rows
+static void wgrad_split(WgradPlan* q, size_t rows, size_t s) {
+    const size_t most = (rows + 63) / 64;
+    s = s < 1 ? 1 : s > most ? most : s;
+    q->rows_per = ((rows + s - 1) / s + 31) / 32 * 32;
+    q->splits = (int)((rows + q->rows_per - 1) / q->rows_per);
+}
+
+// Tile and number of row ranges with the least estimated time: steps of 32 rows times what a step of that tile takes with 1, 2 or 4
+// workgroups on each of 256 CUs (measured, fp32 dy, us), times the rounds, plus the partial results, written and read, and the launch that
+// adds them up.  Over 24 shapes from 512 x 40 x 40 to 65536 x 2048 x 100 the choice is within 9 % of the best of all tiles and splits,
+// 1.5 % on average; the large tile alone would be 1.6 times slower on the small ones (512 x 100 x 100: 17.2 us against 10.8), the
+// small one 1.5 times on the large (65536 x 100 x 2048: 202 us against 125).
 static WgradPlan wgrad_plan(size_t rows, int O, int I) {
     WgradPlan q;
-    int bm, bn, want;
-    if (O <= 32) {
+    if (O <= 32) {  // the codes are the traffic: enough ranges for every CU, more only while each wave has 8 steps of its own
         q.kind = O <= 16 ? WGRAD_NARROW1 : WGRAD_NARROW2;
-        bm = 32;
-        bn = 256;
-        want = WANT_NARROW;
-    } else if (O >= 192 && I >= 192) {
-        q.kind = WGRAD_256;
-        bm = bn = 256;
-        want = 256;
-    } else if (O > 64 && I > 64) {
-        q.kind = WGRAD_128;
-        bm = bn = 128;
-        want = WANT_128;
-    } else {
-        q.kind = WGRAD_64;
-        bm = bn = 64;
-        want = WANT_64;
+        q.tiles_m = 1;
+        q.tiles_n = ceil_div(I, 256);
+        const size_t one = ceil_div(256, q.tiles_n), two = ceil_div(512, q.tiles_n);
+        const size_t s = rows / 1024 > one ? (rows / 1024 < two ? rows / 1024 : two) : one;
+        wgrad_split(&q, rows, s);
+        return q;
     }
-    q.tiles_m = ceil_div(O, bm);
-    q.tiles_n = ceil_div(I, bn);
-    const size_t tiles = (size_t)q.tiles_m * q.tiles_n;
-    size_t s = want / tiles;
-    const size_t most = (rows + MIN_ROWS - 1) / MIN_ROWS;
-    s = s < 1 ? 1 : s > most ? most : s;
-    q.rows_per = ((rows + s - 1) / s + 31) / 32 * 32;
-    q.splits = (int)((rows + q.rows_per - 1) / q.rows_per);
+    static const struct {
+        WgradKind kind;
+        int bm, bn;
+        double first;    // us before the first and after the last step
+        double step[3];  // us a step with 1, 2, 4 workgroups on a CU (0: they do not fit)
+    } tiles[] = {{WGRAD_64, 64, 64, 3., {.75, .88, 1.55}},
+                 {WGRAD_64x256, 64, 256, 5., {1.3, 2.0, 0.}},
+                 {WGRAD_128, 128, 128, 5., {1.45, 2.05, 0.}},
+                 {WGRAD_256, 256, 256, 8., {2.65, 0., 0.}}};
+    double best = 1e300;
+    for (const auto& t : tiles) {
+        WgradPlan c;
+        c.kind = t.kind;
+        c.tiles_m = ceil_div(O, t.bm);
+        c.tiles_n = ceil_div(I, t.bn);
+        const size_t n = (size_t)c.tiles_m * c.tiles_n;
+        for (int want = 128; want <= 1024; want *= 2) {
+            wgrad_split(&c, rows, want / n);
+            const size_t wgs = n * c.splits;
+            int k = 0;
+            while (k < 2 && t.step[k + 1] > 0. && wgs > (256u << k)) ++k;
+            const double rounds = (double)((wgs + (256u << k) - 1) / (256u << k));
+            const double us = t.first + rounds * (double)(c.rows_per / 32) * t.step[k] +
+                              (c.splits > 1 ? 3. + (double)c.splits * O * I * 8. / 4e6 : 0.);
+            if (us < best) {
+                best = us;
+                q = c;
+            }
+        }
+    }
     return q;
 }
 
-template <typename T>
-static void wgrad_launch(WgradKind kind, const WgradP& p, hipStream_t s) {
+template <typename T, bool SIGNED>
+static void wgrad_launch_as(WgradKind kind, const WgradP& p, hipStream_t s) {
     const unsigned grid = (unsigned)p.tiles_m * p.tiles_n * p.splits;
     switch (kind) {
-        case WGRAD_NARROW1: hipLaunchKernelGGL((act8_wgrad_narrow_kernel<T, 1>), dim3(grid), dim3(256), 0, s, p); break;
-        case WGRAD_NARROW2: hipLaunchKernelGGL((act8_wgrad_narrow_kernel<T, 2>), dim3(grid), dim3(256), 0, s, p); break;
-        case WGRAD_64: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, 64, 64, 32, 32>), dim3(grid), dim3(256), 0, s, p); break;
-        case WGRAD_128: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, 128, 128, 64, 64>), dim3(grid), dim3(256), 0, s, p); break;
-        case WGRAD_256: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, 256, 256, 64, 128>), dim3(grid), dim3(512), 0, s, p); break;
+        case WGRAD_NARROW1: hipLaunchKernelGGL((act8_wgrad_narrow_kernel<T, SIGNED, 1>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_NARROW2: hipLaunchKernelGGL((act8_wgrad_narrow_kernel<T, SIGNED, 2>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_64: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, SIGNED, 64, 64, 32, 32>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_64x256: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, SIGNED, 64, 256, 32, 128>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_128: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, SIGNED, 128, 128, 64, 64>), dim3(grid), dim3(256), 0, s, p); break;
+        case WGRAD_256: hipLaunchKernelGGL((act8_wgrad_tile_kernel<T, SIGNED, 256, 256, 64, 128>), dim3(grid), dim3(512), 0, s, p); break;
     }
+}
+
+template <typename T>
+static void wgrad_launch(WgradKind kind, bool rectified, const WgradP& p, hipStream_t s) {
+    if (rectified)
+        wgrad_launch_as<T, false>(kind, p, s);
+    else
+        wgrad_launch_as<T, true>(kind, p, s);
 }
 
 static unsigned stream_grid(size_t vecs) {
@@ -673,13 +733,12 @@ extern "C" int dun_act8_weight_grad(const void* dy, int64_t lddy, const uint8_t*
     p.tiles_m = q.tiles_m;
     p.tiles_n = q.tiles_n;
     p.splits = q.splits;
-    p.zero = relu ? 0.f : 128.f;
     if (dtype == DUN_F32)
-        wgrad_launch<float>(q.kind, p, s);
+        wgrad_launch<float>(q.kind, relu != 0, p, s);
     else if (dtype == DUN_BF16)
-        wgrad_launch<bf16_t>(q.kind, p, s);
+        wgrad_launch<bf16_t>(q.kind, relu != 0, p, s);
     else
-        wgrad_launch<fp16_t>(q.kind, p, s);
+        wgrad_launch<fp16_t>(q.kind, relu != 0, p, s);
     DUN_LAUNCH_CHECK();
     if (need) {
         launch_sum_rows(ws, q.splits, p.stride, dw, n, db, s);
