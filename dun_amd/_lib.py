@@ -215,32 +215,34 @@ def out_ptr(t):
 
 
 
-class _Nothing(object):
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return False
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-_NOTHING = _Nothing()
-
-
-def on_device(t):
-    """Context in which `t`'s device is the current one (kernels launch on the current device)."""
-    if not t.is_cuda:
+def gpu_index(t):
+    """Index of the GPU a tensor is on."""
+    i = t.get_device()
+    if i < 0:
         raise RuntimeError("dun_amd kernels need GPU tensors (got a %s tensor); there is no CPU path" % t.device)
-    if t.device.index == torch.cuda.current_device():
-        return _NOTHING
-    return torch.cuda.device(t.device)
+    return i
+
+
+def elsewhere(i):
+    """None where GPU `i` is the current device (kernels launch on the current device), else a context that makes it so."""
+    return None if i == torch.cuda.current_device() else torch.cuda.device(i)
+
+
+def raw_stream(i):
+    """The current stream of GPU `i` as an integer (stream_ptr without the stream object around it)."""
+    return _raw_stream(i)
 
 
 def rows_view(t):
     """(tensor, row stride) of a 2-D tensor whose rows the kernels can walk: unit column stride, rows that do not overlap;
     anything else (transposed, expanded) is copied."""
     rows, cols = t.shape
+    if t.is_contiguous():
+        return t, cols
     ld = t.stride(0)
     if (t.stride(1) == 1 or cols == 1) and (ld >= cols or rows <= 1):
         return t, (ld if rows > 1 else cols)
-    t = t.contiguous()
-    return t, cols
+    return t.detach().contiguous(), cols

@@ -26,13 +26,18 @@ from . import kernels
 
 def _as_rows(t, what):
     """[..., cols] as a 2-D tensor of rows."""
-    if not isinstance(t, torch.Tensor) or t.dim() < 1:
-        raise RuntimeError("%s must be a tensor of at least one dimension" % what)
+    if not isinstance(t, torch.Tensor):
+        raise RuntimeError("%s must be a tensor (got %s)" % (what, type(t).__name__))
     if t.dtype not in L.ROW_DTYPES:
         raise RuntimeError("%s must be float32, bfloat16 or float16 (got %s)" % (what, t.dtype))
+    if t.dim() != 2:
+        if t.dim() < 1:
+            raise RuntimeError("%s must be a tensor of at least one dimension" % what)
+        if t.shape[-1]:
+            t = t.reshape(-1, t.shape[-1])
     if t.shape[-1] == 0:
         raise RuntimeError("%s has rows of no elements: %s" % (what, tuple(t.shape)))
-    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return t
 
 
 class Packed8(object):
@@ -52,6 +57,14 @@ class Packed8(object):
                 raise RuntimeError("not a checkpoint of a tensor of shape %s: uint8 %s wanted, got %s %s"
                                    % (self.shape, want, t.dtype, tuple(t.shape)))
 
+    @classmethod
+    def _of(cls, packed, shape, relu, dtype):
+        """Around buffers that were made for it (nothing to check)."""
+        p = object.__new__(cls)
+        p.codes, p.exps = packed
+        p.shape, p.relu, p.dtype = tuple(shape), relu, dtype
+        return p
+
     @property
     def packed(self):
         return self.codes, self.exps
@@ -64,14 +77,14 @@ class Packed8(object):
         """The values that the codes stand for (exact in float32 and bfloat16)."""
         if dtype not in L.ROW_DTYPES:
             raise RuntimeError("a checkpoint unpacks to float32, bfloat16 or float16 (got %s)" % dtype)
-        return kernels.backend().act8_unpack(self.packed, self.shape[-1], self.relu, dtype).view(self.shape)
+        v = kernels.backend().act8_unpack((self.codes, self.exps), self.shape[-1], self.relu, dtype)
+        return v if len(self.shape) == 2 else v.view(self.shape)
 
 
 def pack(x, relu=False):
     """The 8-bit checkpoint of ``x`` [..., cols], or of max(x, 0) with ``relu``."""
-    x2 = _as_rows(x.detach(), "pack: x")
-    codes, exps = kernels.backend().act8_pack(x2, bool(relu))
-    return Packed8(codes, exps, x.shape, relu, x.dtype)
+    relu = bool(relu)
+    return Packed8._of(kernels.backend().act8_pack(_as_rows(x, "pack: x"), relu), x.shape, relu, x.dtype)
 
 
 def weight_grad(dy, packed, bias=True):
@@ -79,11 +92,11 @@ def weight_grad(dy, packed, bias=True):
     ``dy`` [..., outs] of its output and the checkpoint of its input.  ``bias=False``: db is None."""
     if not isinstance(packed, Packed8):
         raise RuntimeError("weight_grad: packed must be a Packed8 (got %s)" % type(packed).__name__)
-    dy2 = _as_rows(dy.detach(), "weight_grad: dy")
-    if tuple(dy.shape[:-1]) != packed.shape[:-1] or dy.device != packed.codes.device:
+    dy2 = _as_rows(dy, "weight_grad: dy")
+    if dy.shape[:-1] != packed.shape[:-1] or dy.get_device() != packed.codes.get_device():
         raise RuntimeError("weight_grad: dy %s on %s does not belong to a checkpoint of %s on %s"
                            % (tuple(dy.shape), dy.device, packed.shape, packed.codes.device))
-    return kernels.backend().act8_weight_grad(dy2, packed.packed, packed.shape[-1], packed.relu, want_bias=bool(bias))
+    return kernels.backend().act8_weight_grad(dy2, (packed.codes, packed.exps), packed.shape[-1], packed.relu, bool(bias))
 
 
 class _Linear8(torch.autograd.Function):
@@ -101,7 +114,7 @@ class _Linear8(torch.autograd.Function):
         ctx.save_for_backward(weight, codes, exps)
         if rows == 0:
             return x.new_empty(x.shape[:-1] + (outs,))
-        with L.on_device(x2):
+        with torch.cuda.device(L.gpu_index(x2)):
             y = be.gemm(x2, w, rows, outs, cols, bias=None if bias is None else bias.detach().contiguous())
         return y.view(x.shape[:-1] + (outs,))
 
@@ -117,7 +130,7 @@ class _Linear8(torch.autograd.Function):
             if dy2.shape[0] == 0:
                 dx = dy.new_empty(ctx.shape)
             else:
-                with L.on_device(dy2):
+                with torch.cuda.device(L.gpu_index(dy2)):
                     dx = be.gemm(dy2, weight.detach().contiguous(), dy2.shape[0], cols, outs, b_kcontig=False).view(ctx.shape)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dw, db = be.act8_weight_grad(dy2, (codes, exps), cols, ctx.relu, want_bias=ctx.has_bias)

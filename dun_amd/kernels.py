@@ -472,94 +472,126 @@ class HipBackend(object):
     # them out.  Shapes and types are the callers' business (dun_amd.layer_norm, dun_amd.act8).
     def act8_buffers(self, rows, cols, device):
         groups = (cols + L.ACT8_GROUP - 1) // L.ACT8_GROUP
-        return (torch.empty(rows, groups * L.ACT8_GROUP, device=device, dtype=torch.uint8),
-                torch.empty(rows, groups, device=device, dtype=torch.uint8))
+        return (torch.empty((rows, groups * L.ACT8_GROUP), device=device, dtype=torch.uint8),
+                torch.empty((rows, groups), device=device, dtype=torch.uint8))
 
     def act8_pack(self, x, relu, out=None):
-        with L.on_device(x):
-            x, ld = L.rows_view(x)
-            rows, cols = x.shape
-            codes, exps = self.act8_buffers(rows, cols, x.device) if out is None else out
-            L.check(L.lib().dun_act8_pack(x.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), rows, cols,
-                                          L.ROW_DTYPES[x.dtype], relu, L.stream_ptr(x.device)), "dun_act8_pack")
+        gpu = L.gpu_index(x)
+        ctx = L.elsewhere(gpu)
+        if ctx is not None:
+            with ctx:
+                return self.act8_pack(x, relu, out)
+        x, ld = L.rows_view(x)
+        rows, cols = x.shape
+        codes, exps = self.act8_buffers(rows, cols, x.device) if out is None else out
+        rc = L.lib().dun_act8_pack(x.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), rows, cols, L.ROW_DTYPES[x.dtype], relu,
+                                   L.raw_stream(gpu))
+        if rc:
+            L.check(rc, "dun_act8_pack")
         return codes, exps
 
     def act8_unpack(self, packed, cols, relu, dtype):
         codes, exps = packed
-        with L.on_device(codes):
-            out = torch.empty(codes.shape[0], cols, device=codes.device, dtype=dtype)
-            L.check(L.lib().dun_act8_unpack(codes.data_ptr(), exps.data_ptr(), out.data_ptr(), cols, codes.shape[0], cols,
-                                            L.ROW_DTYPES[dtype], relu, L.stream_ptr(codes.device)), "dun_act8_unpack")
+        gpu = L.gpu_index(codes)
+        ctx = L.elsewhere(gpu)
+        if ctx is not None:
+            with ctx:
+                return self.act8_unpack(packed, cols, relu, dtype)
+        rows = codes.shape[0]
+        out = torch.empty((rows, cols), device=codes.device, dtype=dtype)
+        rc = L.lib().dun_act8_unpack(codes.data_ptr(), exps.data_ptr(), out.data_ptr(), cols, rows, cols, L.ROW_DTYPES[dtype], relu,
+                                     L.raw_stream(gpu))
+        if rc:
+            L.check(rc, "dun_act8_unpack")
         return out
 
     def act8_weight_grad(self, dy, packed, cols, relu, want_bias=True, dw=None, db=None):
         """dw [outs, cols] = dy^T value, db [outs] = sum_rows dy (float32)."""
+        gpu = L.gpu_index(dy)
+        ctx = L.elsewhere(gpu)
+        if ctx is not None:
+            with ctx:
+                return self.act8_weight_grad(dy, packed, cols, relu, want_bias, dw, db)
         codes, exps = packed
         lib = L.lib()
-        with L.on_device(dy):
-            dy, ld = L.rows_view(dy)
-            rows, outs = dy.shape
-            if ld > 1 << 24:  # (the kernels' row stride ends there)
-                dy, ld = dy.contiguous(), outs
-            dt = L.ROW_DTYPES[dy.dtype]
-            f = dict(device=dy.device, dtype=torch.float32)
-            if dw is None:
-                dw = torch.empty(outs, cols, **f)
-            if db is None and want_bias:
-                db = torch.empty(outs, **f)
-            n_ws = lib.dun_act8_weight_grad_workspace_floats(rows, outs, cols, dt)
-            ws = torch.empty(n_ws, **f) if n_ws else None
-            L.check(lib.dun_act8_weight_grad(dy.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), L.f32(dw),
-                                             None if db is None else L.f32(db), None if ws is None else ws.data_ptr(), n_ws,
-                                             rows, outs, cols, dt, relu, L.stream_ptr(dy.device)), "dun_act8_weight_grad")
+        dy, ld = L.rows_view(dy)
+        rows, outs = dy.shape
+        if ld > 1 << 24:  # (the kernels' row stride ends there)
+            dy, ld = dy.detach().contiguous(), outs
+        dt, dev = L.ROW_DTYPES[dy.dtype], dy.device
+        if dw is None:
+            dw = torch.empty((outs, cols), device=dev)
+        if db is None and want_bias:
+            db = torch.empty((outs,), device=dev)
+        n_ws = lib.dun_act8_weight_grad_workspace_floats(rows, outs, cols, dt)
+        ws = torch.empty((n_ws,), device=dev) if n_ws else None
+        rc = lib.dun_act8_weight_grad(dy.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), L.f32(dw), None if db is None else L.f32(db),
+                                      None if ws is None else ws.data_ptr(), n_ws, rows, outs, cols, dt, relu, L.raw_stream(gpu))
+        if rc:
+            L.check(rc, "dun_act8_weight_grad")
         return dw, db
 
     def layer_norm_forward(self, x, w, b, eps, res=None, relu=False, want_stats=True, pack_x=False, pack_y=False, out=None,
                            stats=None, x_packed=None, y_packed=None):
         """-> (y, stats [2, rows] or None, packed z or None, packed y or None); w, b: float32 [cols] or None.  `out` may be
         `res`."""
-        with L.on_device(x):
-            x, ldx = L.rows_view(x)
-            rows, cols = x.shape
-            dev = x.device
-            ldr = 0
-            if res is not None:
-                res, ldr = L.rows_view(res)
-            y = torch.empty(rows, cols, device=dev, dtype=x.dtype) if out is None else out
-            if want_stats and stats is None:
-                stats = torch.empty(2, rows, device=dev, dtype=torch.float32)
-            xq = (self.act8_buffers(rows, cols, dev) if x_packed is None else x_packed) if pack_x else None
-            yq = (self.act8_buffers(rows, cols, dev) if y_packed is None else y_packed) if pack_y else None
-            L.check(L.lib().dun_layer_norm_forward(
-                x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr, None if w is None else w.data_ptr(),
-                None if b is None else b.data_ptr(), y.data_ptr(), cols, None if stats is None else stats.data_ptr(),
-                None if xq is None else xq[0].data_ptr(), None if xq is None else xq[1].data_ptr(),
-                None if yq is None else yq[0].data_ptr(), None if yq is None else yq[1].data_ptr(), rows, cols,
-                L.ROW_DTYPES[x.dtype], eps, relu, L.stream_ptr(dev)), "dun_layer_norm_forward")
+        gpu = L.gpu_index(x)
+        ctx = L.elsewhere(gpu)
+        if ctx is not None:
+            with ctx:
+                return self.layer_norm_forward(x, w, b, eps, res, relu, want_stats, pack_x, pack_y, out, stats, x_packed, y_packed)
+        x, ldx = L.rows_view(x)
+        rows, cols = x.shape
+        ldr = 0
+        if res is not None:
+            res, ldr = L.rows_view(res)
+        y = torch.empty((rows, cols), device=x.device, dtype=x.dtype) if out is None else out
+        if want_stats and stats is None:
+            stats = torch.empty((2, rows), device=x.device)
+        xq = yq = None
+        xc = xe = yc = ye = None
+        if pack_x:
+            xq = self.act8_buffers(rows, cols, x.device) if x_packed is None else x_packed
+            xc, xe = xq[0].data_ptr(), xq[1].data_ptr()
+        if pack_y:
+            yq = self.act8_buffers(rows, cols, x.device) if y_packed is None else y_packed
+            yc, ye = yq[0].data_ptr(), yq[1].data_ptr()
+        rc = L.lib().dun_layer_norm_forward(
+            x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr, None if w is None else w.data_ptr(),
+            None if b is None else b.data_ptr(), y.data_ptr(), cols, None if stats is None else stats.data_ptr(), xc, xe, yc, ye,
+            rows, cols, L.ROW_DTYPES[x.dtype], eps, relu, L.raw_stream(gpu))
+        if rc:
+            L.check(rc, "dun_layer_norm_forward")
         return y, stats, xq, yq
 
     def layer_norm_backward(self, dy, x, packed, w, stats, relu=False, sums=2, dx=None, sums_out=None):
         """-> (dx, sums [sums, cols]: of dy xhat, of dy and, with 3, of dx).  Exactly one of x and packed."""
+        gpu = L.gpu_index(dy)
+        ctx = L.elsewhere(gpu)
+        if ctx is not None:
+            with ctx:
+                return self.layer_norm_backward(dy, x, packed, w, stats, relu, sums, dx, sums_out)
         lib = L.lib()
-        with L.on_device(dy):
-            dy, lddy = L.rows_view(dy)
-            rows, cols = dy.shape
-            dev, dt = dy.device, L.ROW_DTYPES[dy.dtype]
-            ldx = 0
-            if x is not None:
-                x, ldx = L.rows_view(x)
-            if dx is None:
-                dx = torch.empty(rows, cols, device=dev, dtype=dy.dtype)
-            out = torch.empty(sums, cols, device=dev, dtype=torch.float32) if sums and sums_out is None else sums_out
-            n_ws = lib.dun_layer_norm_backward_workspace_floats(rows, cols, dt, sums)
-            ws = torch.empty(n_ws, device=dev, dtype=torch.float32) if n_ws else None
-            codes, exps = (None, None) if packed is None else (packed[0].data_ptr(), packed[1].data_ptr())
-            L.check(lib.dun_layer_norm_backward(
-                dy.data_ptr(), lddy, None if x is None else x.data_ptr(), ldx, codes, exps,
-                None if w is None else w.data_ptr(), stats.data_ptr(), dx.data_ptr(), cols,
-                None if out is None else out.data_ptr(), sums, None if ws is None else ws.data_ptr(), n_ws, rows, cols, dt,
-                relu, L.stream_ptr(dev)), "dun_layer_norm_backward")
-        return dx, out
+        dy, lddy = L.rows_view(dy)
+        rows, cols = dy.shape
+        dev, dt = dy.device, L.ROW_DTYPES[dy.dtype]
+        ldx = 0
+        if x is not None:
+            x, ldx = L.rows_view(x)
+        if dx is None:
+            dx = torch.empty((rows, cols), device=dev, dtype=dy.dtype)
+        if sums and sums_out is None:
+            sums_out = torch.empty((sums, cols), device=dev)
+        n_ws = lib.dun_layer_norm_backward_workspace_floats(rows, cols, dt, sums)
+        ws = torch.empty((n_ws,), device=dev) if n_ws else None
+        codes, exps = (None, None) if packed is None else (packed[0].data_ptr(), packed[1].data_ptr())
+        rc = lib.dun_layer_norm_backward(
+            dy.data_ptr(), lddy, None if x is None else x.data_ptr(), ldx, codes, exps, None if w is None else w.data_ptr(),
+            stats.data_ptr(), dx.data_ptr(), cols, None if sums_out is None else sums_out.data_ptr(), sums,
+            None if ws is None else ws.data_ptr(), n_ws, rows, cols, dt, relu, L.raw_stream(gpu))
+        if rc:
+            L.check(rc, "dun_layer_norm_backward")
+        return dx, sums_out
 
     # ---- raw GEMM (tests / benchmarks) ----------------------------------------------------------------
     def gemm(self, A, B, M, N, K, a_kcontig=True, b_kcontig=True, bias=None, relu=False, R=None, U=None, V=None,

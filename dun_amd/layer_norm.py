@@ -24,34 +24,31 @@ from . import kernels
 from .act8 import Packed8, _as_rows
 
 
-def _vector(t, cols, device, what):
+def _vector(t, cols, x, what):
     """weight / bias as the kernels take it: float32, contiguous."""
-    if t is None:
-        return None
     if t.dim() != 1 or t.shape[0] != cols:
         raise RuntimeError("layer_norm: %s %s does not go with rows of %d elements" % (what, tuple(t.shape), cols))
-    if t.device != device:
-        raise RuntimeError("layer_norm: %s is on %s, x on %s" % (what, t.device, device))
-    if t.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise RuntimeError("layer_norm: %s must be float32, bfloat16 or float16 (got %s)" % (what, t.dtype))
-    t = t.detach()
-    if t.dtype != torch.float32:
-        t = t.float()
-    return t if t.is_contiguous() else t.contiguous()
+    if t.get_device() != x.get_device():
+        raise RuntimeError("layer_norm: %s is on %s, x on %s" % (what, t.device, x.device))
+    if t.dtype is not torch.float32:
+        if t.dtype not in (torch.bfloat16, torch.float16):
+            raise RuntimeError("layer_norm: %s must be float32, bfloat16 or float16 (got %s)" % (what, t.dtype))
+        t = t.detach().float()
+    return t if t.is_contiguous() else t.detach().contiguous()
 
 
 def _checked(x, weight, bias, eps, residual, bits):
     x2 = _as_rows(x, "layer_norm: x")
     cols = x2.shape[1]
-    w = _vector(weight, cols, x.device, "weight")
-    b = _vector(bias, cols, x.device, "bias")
+    w = None if weight is None else _vector(weight, cols, x, "weight")
+    b = None if bias is None else _vector(bias, cols, x, "bias")
     if not eps >= 0:
         raise RuntimeError("layer_norm: eps must not be negative (got %r)" % (eps,))
     if bits not in (None, 8, 32):
         raise RuntimeError("layer_norm: bits is 32 (or None) or 8 (got %r)" % (bits,))
     r2 = None
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.get_device() != x.get_device():
             raise RuntimeError("layer_norm: residual %s %s on %s does not go with x %s %s on %s"
                                % (tuple(residual.shape), residual.dtype, residual.device, tuple(x.shape), x.dtype, x.device))
         r2 = _as_rows(residual, "layer_norm: residual")
@@ -66,38 +63,36 @@ class Saved(object):
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, relu=False, bits=None, pack_output=False):
     """-> (y, saved), or (y, saved, Packed8 of y) with ``pack_output``.  Not recorded by autograd; ``saved`` refers to
     ``x`` itself unless ``bits`` is 8: x must not change before ``layer_norm_backward``."""
-    x = x.detach()
-    x2, w, b, r2 = _checked(x, weight, bias, eps, None if residual is None else residual.detach(), bits)
-    y, stats, xq, yq = kernels.backend().layer_norm_forward(x2, w, b, eps, res=r2, relu=bool(relu), pack_x=bits == 8,
-                                                            pack_y=bool(pack_output))
+    x2, w, b, r2 = _checked(x, weight, bias, eps, residual, bits)
+    relu = bool(relu)
+    y, stats, xq, yq = kernels.backend().layer_norm_forward(x2, w, b, eps, r2, relu, True, bits == 8, bool(pack_output))
     s = Saved()
-    s.x, s.packed, s.w, s.stats, s.relu = (x2 if xq is None else None), xq, w, stats, bool(relu)
+    s.x, s.packed, s.w, s.stats, s.relu = (x2.detach() if xq is None else None), xq, w, stats, relu
     s.shape, s.dtype = x.shape, x.dtype
     s.w_dtype = None if weight is None else weight.dtype
     s.b_dtype = None if bias is None else bias.dtype
     y = y if x.dim() == 2 else y.view(x.shape)
     if pack_output:
-        return y, s, Packed8(yq[0], yq[1], x.shape, False, x.dtype)
+        return y, s, Packed8._of(yq, x.shape, False, x.dtype)
     return y, s
 
 
 def layer_norm_backward(dy, saved, sum_dx=False):
     """-> (dx, dweight, dbias[, sum_rows dx]); the residual's gradient is ``dy``.  dweight / dbias in the types of weight and
     bias (float32 where there was none); with ``sum_dx`` also the float32 bias gradient of the Linear that made x."""
-    if dy.shape != saved.shape or dy.dtype != saved.dtype or dy.device != saved.stats.device:
+    if dy.shape != saved.shape or dy.dtype != saved.dtype or dy.get_device() != saved.stats.get_device():
         raise RuntimeError("layer_norm_backward: dy %s %s on %s does not go with x %s %s on %s"
                            % (tuple(dy.shape), dy.dtype, dy.device, tuple(saved.shape), saved.dtype, saved.stats.device))
-    dy = dy.detach()
     dy2 = dy if dy.dim() == 2 else dy.reshape(-1, dy.shape[-1])
-    dx, sums = kernels.backend().layer_norm_backward(dy2, saved.x, saved.packed, saved.w, saved.stats, relu=saved.relu,
-                                                     sums=3 if sum_dx else 2)
-    dw, db = sums[0], sums[1]
+    dx, sums = kernels.backend().layer_norm_backward(dy2, saved.x, saved.packed, saved.w, saved.stats, saved.relu, 3 if sum_dx else 2)
+    rows = sums.unbind(0)
+    dw, db = rows[0], rows[1]
     if saved.w_dtype not in (None, torch.float32):
         dw = dw.to(saved.w_dtype)
     if saved.b_dtype not in (None, torch.float32):
         db = db.to(saved.b_dtype)
     dx = dx if dy.dim() == 2 else dx.view(saved.shape)
-    return (dx, dw, db, sums[2]) if sum_dx else (dx, dw, db)
+    return (dx, dw, db, rows[2]) if sum_dx else (dx, dw, db)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -126,7 +121,7 @@ class _LayerNorm(torch.autograd.Function):
             s.relu, s.w_dtype, s.b_dtype, s.shape, s.dtype = ctx.info
             s.x = None if x is None else _as_rows(x.detach(), "layer_norm: x")
             s.packed = None if codes is None else (codes, exps)
-            s.w = _vector(weight, s.shape[-1], stats.device, "weight")
+            s.w = None if weight is None else _vector(weight, s.shape[-1], stats, "weight")
             s.stats = stats
             dx, dw, db = layer_norm_backward(dy, s)
         return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dy if need[3] else None,
@@ -136,16 +131,16 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None, relu=False, bits=None, pack_output=False):
     """Layer norm of the rows of ``x`` [..., cols] (see the module's head).  ``pack_output``: -> (y, Packed8 of y), for
     the ``act8.linear`` that reads y next."""
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        x = x.detach()
-        x2, w, b, r2 = _checked(x, weight, bias, eps, None if residual is None else residual.detach(), bits)
-        y, _, _, yq = kernels.backend().layer_norm_forward(x2, w, b, eps, res=r2, relu=bool(relu), want_stats=False,
-                                                           pack_y=bool(pack_output))
+    if not torch.is_grad_enabled() or not (x.requires_grad or (weight is not None and weight.requires_grad)
+                                           or (bias is not None and bias.requires_grad)
+                                           or (residual is not None and residual.requires_grad)):
+        x2, w, b, r2 = _checked(x, weight, bias, eps, residual, bits)
+        y, _, _, yq = kernels.backend().layer_norm_forward(x2, w, b, eps, r2, bool(relu), False, False, bool(pack_output))
         y = y if x.dim() == 2 else y.view(x.shape)
-        return (y, Packed8(yq[0], yq[1], x.shape, False, x.dtype)) if pack_output else y
+        return (y, Packed8._of(yq, x.shape, False, x.dtype)) if pack_output else y
     out = _LayerNorm.apply(x, weight, bias, residual, eps, relu, bits, bool(pack_output))
     if pack_output:
-        return out[0], Packed8(out[1], out[2], x.shape, False, x.dtype)
+        return out[0], Packed8._of((out[1], out[2]), x.shape, False, x.dtype)
     return out
 
 
