@@ -139,7 +139,8 @@ class _Linear8(torch.autograd.Function):
 
 def linear(x, weight, bias=None, packed=None):
     """x weight^T + bias, like torch.nn.functional.linear, keeping ``x`` for the backward in 8 bits.  ``packed``: the
-    checkpoint of ``x`` where the caller has it already (layer_norm's ``pack_output``).  float32."""
+    checkpoint of ``x`` where the caller has it already (layer_norm's ``pack_output``; a rectified checkpoint belongs to a
+    rectified x).  float32."""
     for t, what in ((x, "x"), (weight, "weight"), (bias, "bias")):
         if t is not None and (t.dtype != torch.float32 or t.device != x.device):
             raise RuntimeError("linear: %s must be float32 on %s (got %s on %s)" % (what, x.device, t.dtype, t.device))

@@ -264,8 +264,8 @@ static __global__ __launch_bounds__(256) void sum_few_rows_kernel(const float* p
     }
 }
 static inline void launch_sum_rows(const float* part, size_t P, size_t n, float* out, size_t n1, float* out2, hipStream_t s) {
-    // measured at 128 x 20480: 8 slices 11 us, one 45 us; at 4 x 4.2 M: 32 us, one 21 us
-    if (P <= 8)
+    // rows x elements, us: 8 x 10100 one thread an element 5.7, 8 slices 2.7; 4 x 4.2 M 15 and 32; 128 x 20480 45 and 11
+    if (P <= 8 && n >= (size_t)1 << 18)
         hipLaunchKernelGGL(sum_few_rows_kernel, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s, part, (int)P, n, out, n1, out2);
     else if (P <= 64)
         hipLaunchKernelGGL((sum_rows_kernel<8>), dim3((unsigned)((n + 31) / 32)), dim3(256), 0, s, part, (int)P, n, out, n1, out2);

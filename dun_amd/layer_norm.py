@@ -11,7 +11,9 @@
 forward's mean and rstd.  float32, bfloat16 and float16 rows; statistics and sums in float32; weight and bias of any of these types.
 
 ``layer_norm`` is differentiable (once); ``layer_norm_forward`` / ``layer_norm_backward`` are the two halves for callers
-that run their backward themselves, like the trunks of this package.  Batches couple nowhere: no running statistics, no
+that run their backward themselves, like the trunks of this package.  Both can be captured into a HIP graph.  A captured
+``backward()`` goes by torch's rule for every operator: no earlier autograd graph of the same leaves may be alive (its
+gradient accumulators belong to another stream, which ends the process); the two halves have none.  Batches couple nowhere: no running statistics, no
 exchange between ranks, a batch of one row trains.
 
 The reference's blocks know BatchNorm only (src/DUN/layers.py:33-53).
@@ -77,14 +79,18 @@ def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, relu=
     return y, s
 
 
-def layer_norm_backward(dy, saved, sum_dx=False):
+def layer_norm_backward(dy, saved, sum_dx=False, weight_grads=True):
     """-> (dx, dweight, dbias[, sum_rows dx]); the residual's gradient is ``dy``.  dweight / dbias in the types of weight and
-    bias (float32 where there was none); with ``sum_dx`` also the float32 bias gradient of the Linear that made x."""
+    bias (float32 where there was none), None without ``weight_grads``; with ``sum_dx`` also the float32 bias gradient of
+    the Linear that made x."""
     if dy.shape != saved.shape or dy.dtype != saved.dtype or dy.get_device() != saved.stats.get_device():
         raise RuntimeError("layer_norm_backward: dy %s %s on %s does not go with x %s %s on %s"
                            % (tuple(dy.shape), dy.dtype, dy.device, tuple(saved.shape), saved.dtype, saved.stats.device))
     dy2 = dy if dy.dim() == 2 else dy.reshape(-1, dy.shape[-1])
-    dx, sums = kernels.backend().layer_norm_backward(dy2, saved.x, saved.packed, saved.w, saved.stats, saved.relu, 3 if sum_dx else 2)
+    dx, sums = kernels.backend().layer_norm_backward(dy2, saved.x, saved.packed, saved.w, saved.stats, saved.relu,
+                                                     3 if sum_dx else 2 if weight_grads else 0)
+    if sums is None:
+        return dx if dy.dim() == 2 else dx.view(saved.shape), None, None
     rows = sums.unbind(0)
     dw, db = rows[0], rows[1]
     if saved.w_dtype not in (None, torch.float32):
@@ -123,7 +129,7 @@ class _LayerNorm(torch.autograd.Function):
             s.packed = None if codes is None else (codes, exps)
             s.w = None if weight is None else _vector(weight, s.shape[-1], stats, "weight")
             s.stats = stats
-            dx, dw, db = layer_norm_backward(dy, s)
+            dx, dw, db = layer_norm_backward(dy, s, weight_grads=need[1] or need[2])
         return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dy if need[3] else None,
                 None, None, None, None)
 

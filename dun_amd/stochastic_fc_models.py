@@ -339,6 +339,24 @@ class arq_uncert_fc_MLP(arq_uncert_fc_resnet):
     _block_cls = bern_MLPBlock_nores
 
 
+class _LnFcForward(torch.autograd.Function):
+    """_FcForward for the LayerNorm trunk.  It hangs on a leaf of its own, not on the parameters (whose gradients it writes
+    itself): an act_vec that a caller keeps would otherwise keep the parameters' gradient accumulators alive on its stream, and
+    the backward of a step captured meanwhile would wait for them outside the capture, which ends the process."""
+
+    @staticmethod
+    def forward(ctx, model, x, depth, leaf):
+        buf = model._run_forward(x, depth, True)
+        ctx.model, ctx.buf, ctx.generation = model, buf, buf.generation
+        act, buf.act = buf.act, None  # (a reference cycle through the C++ graph otherwise, as in _FcForward)
+        return act
+
+    @staticmethod
+    def backward(ctx, dact):
+        _FcForward.backward(ctx, dact)
+        return None, None, None, None
+
+
 class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
     """The residual trunk with LayerNorm in its blocks, h + LayerNorm(ReLU(Linear(h))): no counterpart in the reference,
     whose blocks normalise over the batch (src/DUN/layers.py:33-42).
@@ -359,6 +377,14 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
 
     def _flatten_norm(self, dev):
         return None, None, None
+
+    def forward(self, x, depth=None, objective=None):
+        if self.training and torch.is_grad_enabled() and any(p.requires_grad for p in self._param_list):
+            return _LnFcForward.apply(self, x, self.n_layers if depth is None else depth, self.flat_params.new_empty(0).requires_grad_())
+        with torch.no_grad():
+            return super(arq_uncert_fc_resnet_ln, self).forward(x, depth, objective)
+
+    forward_get_acts = forward
 
     def _make_buffers(self, B, depth, train):
         return kernels.backend().ln_fc_buffers(self, B, depth, train)

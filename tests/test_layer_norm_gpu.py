@@ -275,3 +275,51 @@ def test_more_than_2_31_elements():
     dx, dw, db = layer_norm_backward(x, saved)
     within(dx[-3:], o.dx, o.dx_tol, "dx")
     within(dw, o.dw, o.dw_tol * 4, "dw")  # (the other rows add exact zeros)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (5, 33), (300, 100), (40, 1031), (9, 9000)])
+@pytest.mark.parametrize("bits", [None, 8])
+def test_dx_alone(rows, cols, bits):
+    x, w, b, res, dy = make(rows, cols, F32, 31)
+    o = Norm(x, w, b, 1e-5, res, True, bits).backward(dy)
+    y = layer_norm(x.requires_grad_(), w, b, 1e-5, res, True, bits)
+    within(torch.autograd.grad(y, x, dy, retain_graph=True)[0], o.dx, o.dx_tol, "dx")
+    r2 = res.clone().requires_grad_()
+    y = layer_norm(x.detach(), w, b, 1e-5, r2, True, bits)
+    assert torch.equal(torch.autograd.grad(y, r2, dy)[0], dy)
+
+
+def test_output_in_place_of_the_residual_and_gradient_in_place():
+    from dun_amd import kernels
+    be = kernels.backend()
+    for cols in (3, 33, 1031, 2049, 9001):
+        x, w, b, res, dy = make(50, cols, F32, cols)
+        want, saved = layer_norm_forward(x, w, b, 1e-5, res, True)
+        dx = layer_norm_backward(dy, saved)[0]
+        y, stats, _, _ = be.layer_norm_forward(x, w, b, 1e-5, res, True, out=res)
+        got, _ = be.layer_norm_backward(dy, x, None, w, stats, True, 2, dx=dy)
+        assert torch.equal(y, want) and torch.equal(got, dx)
+
+
+def test_autograd_under_capture():
+    x, w, b, res, dy = make(128, 200, F32, 33)
+    leaves = [t.requires_grad_() for t in (x, w, b, res)]
+
+    def step():
+        y = layer_norm(*leaves[:3], 1e-5, leaves[3], True, 8)
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for _ in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(held, step()))

@@ -213,3 +213,27 @@ def test_the_toy_command_trains_it(bits, tmp_path):
     r = subprocess.run([sys.executable, "examples/train_toy.py", "--n_epochs", "6", "--network", "ResNetLN", "--act_bits", bits, "--N_layers", "3",
                         "--width", "32", "--savedir", str(tmp_path)], capture_output=True, text=True, timeout=110)
     assert r.returncode == 0 and "final ELBO estimate" in r.stdout, r.stderr[-2000:]
+
+
+def test_a_kept_act_vec_does_not_disturb_a_captured_step():
+    x, y = O.synthetic_regression(200, 13, seed=7)
+    runs = []
+    for keep in (False, True):
+        net = build(bits=8)
+        net.model.train()
+        kept = net.model(torch.as_tensor(x).cuda()) if keep else None
+        runs.append([net.fit(x, y) for _ in range(4)])
+        assert any(s["graph"] is not None for s in net._graph_states.values())
+        if keep:
+            with pytest.raises(RuntimeError, match="reused by a later"):
+                kept.sum().backward()
+    assert runs[0] == runs[1]
+
+
+def test_frozen_parameters_need_no_gradient():
+    m = build().model.train()
+    x = torch.randn(8, 13, device="cuda")
+    assert m(x).requires_grad
+    for p in m.parameters():
+        p.requires_grad_(False)
+    assert not m(x).requires_grad
