@@ -463,7 +463,8 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_backward_long_kernel(const
 // Teams and vectors of four elements per lane, by the elements that a team holds: the fewest lanes up to a wave, then more vectors per
 // lane, then more waves.  What decides is the bytes in flight: few registers per row for many rows at a time, but no idle lanes.
 // 65536 x 2048 fp32, forward / backward: 64 x 8 237 / 330 us, 256 x 2 200 / 297 us (a plain copy of as many bytes: 208 / 312);
-// 16391 x 1031 bf16: 256 x 2, half of its lanes idle, 34 / 60 us, 128 x 3 27 / 43 us.
+// 16391 x 1031 bf16: 256 x 2, half of its lanes idle, 34 / 60 us, 128 x 3 26 / 38 us.  512 x 8 for rows of up to 16384 elements spills: 2000 x
+// 16384 fp32 96 / 163 us, walked in memory 75 / 235 us.
 #define DUN_LN_TEAMS(X) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(64, 2) X(64, 3) X(64, 4) X(128, 3) X(256, 2) X(256, 4) X(1024, 2)
 
 static int ln_team(int cols, int* ch) {
@@ -479,15 +480,18 @@ static int ln_team(int cols, int* ch) {
     return 0;  // too long for registers
 }
 
-// Workgroups of a backward pass, each with a partial row of sums: what 256 CUs hold at once, no more than there are rows (65536 x 2048
-// fp32 from the checkpoint: 768 243 us, 1024 231 us, 1536 278 us)
+// Workgroups of a backward pass, each with a partial row of sums: as many as 256 CUs hold at once (by the registers of the team's rows; a second
+// round costs as much as it brings: 65536 x 2048 fp32 from the checkpoint: 512 272 us, 1024 230 us, 1536 256 us), and two rows a team
+// before more workgroups (4099 x 517: 1025 15.7 us, 513 11.7 us)
 static size_t ln_backward_blocks(size_t rows, int cols) {
     int ch;
     const int team = ln_team(cols, &ch);
     if (team == 0) return rows < 256 ? rows : 256;
     const size_t tpb = team <= 64 ? 256 / team : 1;
     const size_t need = (rows + tpb - 1) / tpb;
-    return need < 1024 ? need : 1024;
+    const size_t most = team == 1024 ? 256 : team == 256 ? (ch == 2 ? 1024 : 512) : team == 128 ? 1536 : ch <= 2 ? 1024 : ch == 3 ? 768 : 512;
+    const size_t half = need <= 512 ? need : need <= 1024 ? 512 : (need + 1) / 2;
+    return half < most ? half : most;
 }
 
 template <typename T>
