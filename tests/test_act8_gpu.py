@@ -262,3 +262,31 @@ def test_more_than_2_31_elements():
     d, v = dy[-2:].cpu().double(), values_of(x[-2:], False)
     within(dw, d.t() @ v, grad_bound(d, v, 2), "dw")
     assert torch.equal(p.unpack(BF16)[-2:].cpu().double(), v)
+
+
+@pytest.mark.parametrize("outs", [3, 40])
+def test_weight_grad_of_tiny_gradients(outs):
+    # a part of dy that is below bf16's smallest number, 2^-133, is lost, no more: |error| <= 2^-133 |value| on top of rounding
+    v = torch.full((1, 32), 2.0 ** 100)
+    p = act8.pack(v.cuda())
+    for k in (-100, -110, -118, -125):
+        dy = (1 + rand(1, outs, seed=30).abs()) * 2.0 ** k
+        dw, _ = act8.weight_grad(dy.cuda(), p)
+        want = dy.double().t() @ v.double()
+        within(dw, want, 4 * U32 * want.abs() + 2.0 ** -133 * 2.0 ** 100, "dw at 2^%d" % k)
+
+
+def test_weight_grad_keeps_out_what_lies_behind_the_rows():
+    # rows of a longer tensor, NaN behind them and beside them: neither is read into the result
+    for rows in (1, 5, 31, 33, 70, 95, 1000):
+        big = torch.full((rows + 40, 60), float("nan"), device="cuda")
+        big[:rows, 4:50] = rand(rows, 46, seed=rows).cuda()
+        x = torch.full((rows + 40, 70), float("nan"), device="cuda")
+        x[:rows] = rand(rows, 70, seed=31).cuda()
+        whole = act8.pack(x)
+        p = act8.Packed8(whole.codes[:rows], whole.exps[:rows], (rows, 70), False, F32)
+        for dy in (big[:rows, 4:50], big[:rows, 10:13]):
+            dw, db = act8.weight_grad(dy, p)
+            d, v = dy.cpu().double(), p.unpack().cpu().double()
+            within(dw, d.t() @ v, grad_bound(d, v, rows), "dw")
+            within(db, d.sum(0), (rows + 64) * U32 * d.abs().sum(0) + 1e-37, "db")
