@@ -4,7 +4,7 @@ import torch
 
 from dun_amd import act8
 from dun_amd.layer_norm import LayerNorm, layer_norm, layer_norm_backward, layer_norm_forward
-from tests.row_oracle import Norm, codes_of, within
+from tests.row_oracle import Norm, U32, codes_of, within
 
 pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
@@ -323,3 +323,17 @@ def test_autograd_under_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(held, step()))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("relu", [False, True])
+def test_rows_of_one_element(dtype, relu):
+    # the element is its own mean: y = bias, and g - mean(g) = 0 exactly whatever the rounding of g = dy weight is
+    x = torch.randn(37, 1, device="cuda").to(dtype)
+    dy = torch.randn(37, 1, device="cuda").to(dtype)
+    w, b = torch.tensor([1.1], device="cuda"), torch.tensor([0.375], device="cuda")
+    y, saved = layer_norm_forward(x, w, b, 1e-5, relu=relu)
+    dx, dw, db, ds = layer_norm_backward(dy, saved, sum_dx=True)
+    assert torch.equal(y, torch.full_like(y, 0.375))
+    assert torch.equal(dx, torch.zeros_like(dx)) and torch.equal(dw, torch.zeros_like(dw)) and torch.equal(ds, torch.zeros_like(ds))
+    within(db, dy.double().cpu().sum(0), 128 * U32 * dy.double().cpu().abs().sum(0), "db")
