@@ -89,7 +89,8 @@ def pack(x, relu=False):
 
 def weight_grad(dy, packed, bias=True):
     """(dw [outs, cols], db [outs]): the float32 gradients of the weight and bias of a Linear layer, from the gradient
-    ``dy`` [..., outs] of its output and the checkpoint of its input.  ``bias=False``: db is None."""
+    ``dy`` [..., outs] of its output and the checkpoint of its input.  ``bias=False``: db is None.  An infinity in a float32 or
+    float16 ``dy`` counts as NaN for its output's weights (its parts are infinity and NaN)."""
     if not isinstance(packed, Packed8):
         raise RuntimeError("weight_grad: packed must be a Packed8 (got %s)" % type(packed).__name__)
     dy2 = _as_rows(dy, "weight_grad: dy")
@@ -101,14 +102,14 @@ def weight_grad(dy, packed, bias=True):
 
 class _Linear8(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, packed):
+    def forward(ctx, x, weight, bias, packed, keep):
         be = kernels.backend()
         x2 = x.detach().reshape(-1, x.shape[-1]).contiguous()
         w = weight.detach().contiguous()
         rows, cols, outs = x2.shape[0], x2.shape[1], w.shape[0]
         ctx.shape, ctx.has_bias, ctx.relu = tuple(x.shape), bias is not None, False
         codes = exps = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+        if keep:
             codes, exps = be.act8_pack(x2, False) if packed is None else packed.packed
             ctx.relu = False if packed is None else packed.relu
         ctx.save_for_backward(weight, codes, exps)
@@ -134,7 +135,7 @@ class _Linear8(torch.autograd.Function):
                     dx = be.gemm(dy2, weight.detach().contiguous(), dy2.shape[0], cols, outs, b_kcontig=False).view(ctx.shape)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dw, db = be.act8_weight_grad(dy2, (codes, exps), cols, ctx.relu, want_bias=ctx.has_bias)
-        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None
+        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None, None
 
 
 def linear(x, weight, bias=None, packed=None):
@@ -150,7 +151,9 @@ def linear(x, weight, bias=None, packed=None):
         raise RuntimeError("linear: bias %s does not go with weight %s" % (tuple(bias.shape), tuple(weight.shape)))
     if packed is not None and (not isinstance(packed, Packed8) or packed.shape != tuple(x.shape) or packed.codes.device != x.device):
         raise RuntimeError("linear: packed is not a checkpoint of x %s" % (tuple(x.shape),))
-    return _Linear8.apply(x, weight, bias, packed)
+    # (needs_input_grad does not know of no_grad: a prediction would pack what nothing reads)
+    keep = torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad))
+    return _Linear8.apply(x, weight, bias, packed, keep)
 
 
 class Linear(nn.Linear):

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from dun_amd import act8
+from dun_amd import act8, kernels
 from dun_amd.layer_norm import layer_norm
 from tests.row_oracle import U32, codes_of, values_of, within
 
@@ -290,3 +290,41 @@ def test_weight_grad_keeps_out_what_lies_behind_the_rows():
             d, v = dy.cpu().double(), p.unpack().cpu().double()
             within(dw, d.t() @ v, grad_bound(d, v, rows), "dw")
             within(db, d.sum(0), (rows + 64) * U32 * d.abs().sum(0) + 1e-37, "db")
+
+
+@pytest.mark.parametrize("outs", [3, 40, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_weight_grad_of_gradients_that_are_not_finite(outs, dtype, bad):
+    # an infinity counts as NaN (bfloat16, which is not taken apart: as itself); only its own output sees it, and the bias exactly
+    x = rand(70, 40, seed=32)
+    x[33, 5] = 0
+    dy = rand(70, outs, seed=33).to(dtype)
+    dy[33, 1] = bad
+    p = act8.pack(x.cuda())
+    dw, db = act8.weight_grad(dy.cuda(), p)
+    d, v = dy.double(), p.unpack().cpu().double()
+    want = bad * v[33] if dtype == BF16 else torch.full((40,), float("nan"), dtype=torch.float64)
+    as_numbers = lambda t: torch.nan_to_num(t.cpu().double(), 7.0, 8.0, 9.0)
+    assert torch.equal(as_numbers(dw[1]), as_numbers(want))
+    assert torch.equal(as_numbers(db[1]), as_numbers(torch.tensor(bad)))
+    rest = [o for o in range(outs) if o != 1]
+    within(dw[rest], d[:, rest].t() @ v, grad_bound(d[:, rest], v, 70), "dw")
+    within(db[rest], d[:, rest].sum(0), (70 + 64) * U32 * d[:, rest].abs().sum(0) + 1e-37, "db")
+
+
+def test_linear_packs_only_what_a_backward_reads(monkeypatch):
+    x, layer = rand(64, 48, seed=34).cuda(), act8.Linear(48, 20).cuda()
+    want = layer(x)
+    calls = []
+    pack = kernels.HipBackend.act8_pack
+    monkeypatch.setattr(kernels.HipBackend, "act8_pack", lambda *a, **k: (calls.append(1), pack(*a, **k))[1])
+    with torch.no_grad():
+        assert torch.equal(layer(x), want) and not calls
+    with torch.inference_mode():
+        assert torch.equal(layer(x), want) and not calls
+    frozen = act8.linear(x.clone().requires_grad_(), layer.weight.detach(), layer.bias.detach())
+    frozen.sum().backward()
+    assert torch.equal(frozen, want) and not calls
+    layer(x).sum().backward()
+    assert len(calls) == 1
