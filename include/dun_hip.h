@@ -444,8 +444,8 @@ int dun_copy_pair_indirect(void* dst0, size_t bytes0, void* dst1, size_t bytes1,
 #define DUN_F16 2
 
 /* z = x, or max(x, 0) with relu; y = [res +] (z - mean) / sqrt(var + eps) * w + b over each row (biased variance).
- * w, b [cols], each nullable (1, 0).  stats float [2][rows] (nullable): mean, 1 / sqrt(var + eps), what backward needs.
- * x_codes / x_exps (nullable): the checkpoint of z, rectified with relu; y_codes / y_exps (nullable): of y, signed. */
+ * y may be res.  w, b [cols], each nullable (1, 0).  stats float [2][rows] (nullable): mean, 1 / sqrt(var + eps), what
+ * backward needs.  x_codes / x_exps (nullable): the checkpoint of z, rectified with relu; y_codes / y_exps (nullable): of y, signed. */
 int dun_layer_norm_forward(const void* x, int64_t ldx, const void* res, int64_t ldr, const float* w, const float* b, void* y,
                            int64_t ldy, float* stats, uint8_t* x_codes, uint8_t* x_exps, uint8_t* y_codes, uint8_t* y_exps,
                            int64_t rows, int cols, int dtype, float eps, int relu, dun_stream_t stream);
