@@ -15,8 +15,8 @@
 // kernel: no atomics, the same bits every time.
 //
 // 65536 x 2048 fp32: forward 200 us, backward 300 us, 5.4 TB/s both (a copy of 1 GiB: 5.2); the residual block with its checkpoint
-// 300 us and, from the codes, 230 us (5.8, 5.3 TB/s).  16391 x 1031 bf16, where rows start anywhere: 26 and 38 us (2.6 TB/s): too few
-// bytes in flight, a row of 2 KB on two waves.  Small ones are launches: 512 x 100 fp32 4.2 + 4.4 + 2.7 us.
+// 300 us and, from the codes, 218 us (5.8, 5.6 TB/s).  16391 x 1031 bf16, where rows start anywhere: 28 and 29 us (2.4, 3.5 TB/s): too
+// few bytes in flight, a row of 2 KB on two waves.  Small ones are launches: 512 x 100 fp32 4.2 + 4.4 + 2.7 us.
 #include "rows.h"
 
 namespace dun {
@@ -247,8 +247,8 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnB
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[k][c][e] = 0.f;
     // A lane sees the same columns in every row.  Weights that stay in registers spare each row a wait for the cache:
-    // with them in 16-bit rows 65536 x 2048 takes 183 us and not 196, in fp32 rows with 8-bit codes 16384 x 4096 takes
-    // 117 us and not 122.  Plain fp32 rows are bound by memory and want the waves instead: 310 us at 65536 x 2048 with
+    // with them in 16-bit rows 16391 x 1031 takes 29 us and not 38, in fp32 rows with 8-bit codes 65536 x 2048 takes
+    // 218 us and not 237.  Plain fp32 rows are bound by memory and want the waves instead: 310 us at 65536 x 2048 with
     // the weights read row by row, 338 with them kept.
     constexpr bool KEEP_W = MASK || sizeof(T) < 4;
     RawVec<float> w[CH];
@@ -479,7 +479,7 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_backward_long_kernel(const
 // Teams and vectors of four elements per lane, by the elements that a team holds: the fewest lanes up to a wave, then more vectors per
 // lane, then more waves.  What decides is the bytes in flight: few registers per row for many rows at a time, but no idle lanes.
 // 65536 x 2048 fp32, forward / backward: 64 x 8 237 / 330 us, 256 x 2 200 / 297 us (a plain copy of as many bytes: 208 / 312);
-// 16391 x 1031 bf16: 256 x 2, half of its lanes idle, 34 / 60 us, 128 x 3 26 / 38 us.  512 x 8 for rows of up to 16384 elements spills: 2000 x
+// 16391 x 1031 bf16: 256 x 2, half of its lanes idle, 34 / 60 us, 128 x 3 26 / 38 us (since: 28 / 29).  512 x 8 for rows of up to 16384 elements spills: 2000 x
 // 16384 fp32 96 / 163 us, walked in memory 75 / 235 us.
 #define DUN_LN_TEAMS(X) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(64, 2) X(64, 3) X(64, 4) X(128, 3) X(256, 2) X(256, 4) X(1024, 2)
 
@@ -497,7 +497,7 @@ static int ln_team(int cols, int* ch) {
 }
 
 // Workgroups of a backward pass, each with a partial row of sums: as many as 256 CUs hold at once (by the registers of the team's rows; a second
-// round costs as much as it brings: 65536 x 2048 fp32 from the checkpoint: 512 272 us, 1024 230 us, 1536 256 us), and two rows a team
+// round costs as much as it brings: 65536 x 2048 fp32 from the checkpoint: 512 272 us, 1024 230 us (218 since), 1536 256 us), and two rows a team
 // before more workgroups (4099 x 517: 1025 15.7 us, 513 11.7 us)
 static size_t ln_backward_blocks(size_t rows, int cols) {
     int ch;
@@ -517,7 +517,7 @@ static void ln_launch_forward(const LnFwdP& p, hipStream_t s) {
     const int team = ln_team(p.cols, &ch);
     const size_t tpb = team && team <= 64 ? 256 / team : 1;
     const size_t need = (p.rows + tpb - 1) / tpb;
-        const dim3 grid((unsigned)(need < (1u << 20) ? need : (1u << 20)));
+    const dim3 grid((unsigned)(need < (1u << 20) ? need : (1u << 20)));
 #define DUN_LN_FWD(TEAM, CH)                                                                               \
     if (team == TEAM && ch == CH) {                                                                        \
         hipLaunchKernelGGL((ln_forward_kernel<T, TEAM, CH>), grid, dim3(ln_block<TEAM>()), 0, s, p);       \
