@@ -239,6 +239,7 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnB
     TeamSum<TEAM> sum(red);
     const int t = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
     const float n = (float)p.cols, floor_ = MASK && p.relu ? 0.f : -INFINITY;
+    const float dead = MASK && p.relu ? 0.f : NAN;  // z <= dead has no gradient; without ReLU none, -inf not either
     float acc[K > 0 ? K : 1][CH][E];
 #pragma unroll
     for (int k = 0; k < K; ++k)
@@ -312,7 +313,7 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnB
             for (int e = 0; e < E; ++e) {
                 const float xhat = MASK ? (h[c][e] - mean) * rstd : h[c][e];
                 o[e] = rstd * (g[c][e] - s1 - xhat * s2);
-                if (MASK) o[e] = h[c][e] <= floor_ ? 0.f : o[e];
+                if (MASK) o[e] = h[c][e] <= dead ? 0.f : o[e];
                 if (K > 2) acc[K > 2 ? 2 : 0][c][e] += c < ln_whole<TEAM, CH>() || i0 + e < p.cols ? o[e] : 0.f;
             }
             store_part(dx, i0, p.cols, o);

@@ -337,3 +337,14 @@ def test_rows_of_one_element(dtype, relu):
     assert torch.equal(y, torch.full_like(y, 0.375))
     assert torch.equal(dx, torch.zeros_like(dx)) and torch.equal(dw, torch.zeros_like(dw)) and torch.equal(ds, torch.zeros_like(ds))
     within(db, dy.double().cpu().sum(0), 128 * U32 * dy.double().cpu().abs().sum(0), "db")
+
+
+@pytest.mark.parametrize("cols", [7, 100, 517, 2048, 9000])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_row_that_is_not_finite_has_no_gradient_anywhere(cols, bad):
+    x, w, b, _, dy = make(3, cols, F32, 7)
+    x[1, cols // 2] = bad
+    _, saved = layer_norm_forward(x, w, b, 1e-5)
+    for kw in ({}, {"sum_dx": True}, {"weight_grads": False}):
+        dx = layer_norm_backward(dy, saved, **kw)[0]
+        assert torch.isnan(dx[1]).all() and torch.isfinite(dx[0]).all() and torch.isfinite(dx[2]).all(), kw
