@@ -520,11 +520,11 @@ class HipBackend(object):
             dy, ld = dy.detach().contiguous(), outs
         dt, dev = L.ROW_DTYPES[dy.dtype], dy.device
         if dw is None:
-            dw = torch.empty((outs, cols), device=dev)
+            dw = torch.empty((outs, cols), device=dev, dtype=torch.float32)
         if db is None and want_bias:
-            db = torch.empty((outs,), device=dev)
+            db = torch.empty((outs,), device=dev, dtype=torch.float32)
         n_ws = lib.dun_act8_weight_grad_workspace_floats(rows, outs, cols, dt)
-        ws = torch.empty((n_ws,), device=dev) if n_ws else None
+        ws = torch.empty((n_ws,), device=dev, dtype=torch.float32) if n_ws else None
         rc = lib.dun_act8_weight_grad(dy.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), L.f32(dw), None if db is None else L.f32(db),
                                       None if ws is None else ws.data_ptr(), n_ws, rows, outs, cols, dt, relu, L.raw_stream(gpu))
         if rc:
@@ -547,7 +547,7 @@ class HipBackend(object):
             res, ldr = L.rows_view(res)
         y = torch.empty((rows, cols), device=x.device, dtype=x.dtype) if out is None else out
         if want_stats and stats is None:
-            stats = torch.empty((2, rows), device=x.device)
+            stats = torch.empty((2, rows), device=x.device, dtype=torch.float32)
         xq = yq = None
         xc = xe = yc = ye = None
         if pack_x:
@@ -558,7 +558,7 @@ class HipBackend(object):
             yc, ye = yq[0].data_ptr(), yq[1].data_ptr()
         rc = L.lib().dun_layer_norm_forward(
             x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr, None if w is None else w.data_ptr(),
-            None if b is None else b.data_ptr(), y.data_ptr(), cols, None if stats is None else stats.data_ptr(), xc, xe, yc, ye,
+            None if b is None else b.data_ptr(), y.data_ptr(), cols, None if stats is None else L.f32(stats), xc, xe, yc, ye,
             rows, cols, L.ROW_DTYPES[x.dtype], eps, relu, L.raw_stream(gpu))
         if rc:
             L.check(rc, "dun_layer_norm_forward")
@@ -581,13 +581,13 @@ class HipBackend(object):
         if dx is None:
             dx = torch.empty((rows, cols), device=dev, dtype=dy.dtype)
         if sums and sums_out is None:
-            sums_out = torch.empty((sums, cols), device=dev)
+            sums_out = torch.empty((sums, cols), device=dev, dtype=torch.float32)
         n_ws = lib.dun_layer_norm_backward_workspace_floats(rows, cols, dt, sums)
-        ws = torch.empty((n_ws,), device=dev) if n_ws else None
+        ws = torch.empty((n_ws,), device=dev, dtype=torch.float32) if n_ws else None
         codes, exps = (None, None) if packed is None else (packed[0].data_ptr(), packed[1].data_ptr())
         rc = lib.dun_layer_norm_backward(
             dy.data_ptr(), lddy, None if x is None else x.data_ptr(), ldx, codes, exps, None if w is None else w.data_ptr(),
-            stats.data_ptr(), dx.data_ptr(), cols, None if sums_out is None else sums_out.data_ptr(), sums,
+            L.f32(stats), dx.data_ptr(), cols, None if sums_out is None else L.f32(sums_out), sums,
             None if ws is None else ws.data_ptr(), n_ws, rows, cols, dt, relu, L.raw_stream(gpu))
         if rc:
             L.check(rc, "dun_layer_norm_backward")
