@@ -6,6 +6,8 @@ and its backward runs in the HIP trunk kernels (dun_amd/csrc/trunk.hip, gemm.hip
 parameters are views into one flat fp32 buffer that the kernels, the fused SGD step and the gradient
 all-reduce address directly; gradients land in a second flat buffer whose views are the parameters' ``.grad``.
 """
+import weakref
+
 import torch
 import torch.nn as nn
 
@@ -340,9 +342,11 @@ class arq_uncert_fc_MLP(arq_uncert_fc_resnet):
 
 
 class _LnFcForward(torch.autograd.Function):
-    """_FcForward for the LayerNorm trunk.  It hangs on a leaf of its own, not on the parameters (whose gradients it writes
-    itself): an act_vec that a caller keeps would otherwise keep the parameters' gradient accumulators alive on its stream, and
-    the backward of a step captured meanwhile would wait for them outside the capture, which ends the process."""
+    """_FcForward for a step whose backward holds no other term of the parameters (the wrappers' captured step).  It hangs on a
+    leaf of its own, not on the parameters (whose gradients it writes itself): an act_vec that a caller keeps from before keeps
+    the parameters' gradient accumulators alive on its stream, and the backward of a captured step that hung on them would wait for
+    them outside the capture, which ends the process.  Next to other terms this node would be wrong: nothing makes autograd run it
+    before it adds their gradients, which the trunk's backward then overwrites."""
 
     @staticmethod
     def forward(ctx, model, x, depth, leaf):
@@ -368,6 +372,7 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
     Same wrappers, flat parameters, optimiser and checkpoints as the BatchNorm trunk.  Weights in float32."""
     _block_cls = bern_LNBlock
     supports_head_objective = False
+    _step_alone = False  # set by the wrappers around a captured step
 
     def __init__(self, input_dim, output_dim, width, n_layers, w_prior=None, BMA_prior=False, act_bits=32):
         if act_bits not in (8, 32):
@@ -375,14 +380,32 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
         super(arq_uncert_fc_resnet_ln, self).__init__(input_dim, output_dim, width, n_layers, w_prior, BMA_prior)
         self.act_bits, self.ln_eps = act_bits, 1e-5
 
+    def _flatten(self):
+        super(arq_uncert_fc_resnet_ln, self)._flatten()
+        if "_nodes" not in self.__dict__:  # autograd nodes of forwards that are still alive: the stream they ran on
+            self._nodes = weakref.WeakKeyDictionary()
+
+    def __getstate__(self):
+        st = super(arq_uncert_fc_resnet_ln, self).__getstate__()
+        st.pop("_nodes", None)
+        return st
+
     def _flatten_norm(self, dev):
         return None, None, None
 
     def forward(self, x, depth=None, objective=None):
-        if self.training and torch.is_grad_enabled() and any(p.requires_grad for p in self._param_list):
+        if not (self.training and torch.is_grad_enabled() and any(p.requires_grad for p in self._param_list)):
+            with torch.no_grad():
+                return super(arq_uncert_fc_resnet_ln, self).forward(x, depth, objective)
+        if self._step_alone:
             return _LnFcForward.apply(self, x, self.n_layers if depth is None else depth, self.flat_params.new_empty(0).requires_grad_())
-        with torch.no_grad():
-            return super(arq_uncert_fc_resnet_ln, self).forward(x, depth, objective)
+        stream = torch.cuda.current_stream(self.flat_params.device).cuda_stream if self.flat_params.is_cuda else 0
+        if stream and torch.cuda.is_current_stream_capturing() and any(s != stream for s in list(self._nodes.values())):
+            raise RuntimeError("an act_vec from before this capture is still alive: its graph holds the parameters' gradient "
+                               "accumulators on another stream, and a captured backward would wait for them there; drop it first")
+        act = super(arq_uncert_fc_resnet_ln, self).forward(x, depth, objective)
+        self._nodes[act.grad_fn] = stream
+        return act
 
     forward_get_acts = forward
 

@@ -246,6 +246,8 @@ class DUN(BaseNet):
             indirect = getattr(be, "copy_pair_indirect", None)
             torch.cuda.synchronize()
             self._metrics_out = pinned
+            # (no weight prior here, see _graph_key: the trunk's backward is the step's only one that reaches the parameters)
+            self.model._step_alone = True
             try:
                 with torch.cuda.graph(graph):
                     if indirect is not None:
@@ -257,6 +259,7 @@ class DUN(BaseNet):
                         host.copy_(m, non_blocking=True)
             finally:
                 self._metrics_out = None
+                del self.model._step_alone
             # the graph holds raw pointers into the trunk's activation buffers: keep them alive as long as the graph
             # (the model's buffer cache evicts on its own schedule)
             keep = list(getattr(self.model, "_fc_cache", {}).values())
