@@ -7,6 +7,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DUN_HIP_LIB") or os.path.join(_HERE, "libdun_hip.so")
@@ -223,7 +224,21 @@ def gpu_index(t):
     i = t.get_device()
     if i < 0:
         raise RuntimeError("dun_amd kernels need GPU tensors (got a %s tensor); there is no CPU path" % t.device)
+    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and _recorded()):
+        # (a recording would hold the allocation of the output and not the kernel that fills it)
+        raise RuntimeError("dun_amd kernels are not operators of a recorded graph (torch.jit.trace, make_fx); capture a HIP graph")
     return i
+
+
+def _recorded():
+    from torch.fx.experimental.proxy_tensor import get_proxy_mode
+    return get_proxy_mode() is not None
+
+
+def no_tangents(what, *tensors):
+    """Refuses tensors that carry a forward-mode derivative: the kernels have none, and the result would look like a constant."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("%s has no forward-mode derivative (backward() only)" % what)
 
 
 def elsewhere(i):

@@ -14,6 +14,9 @@ A group that holds an infinity or a NaN, or whose largest magnitude would round 
 gradient the exact sum of three, so the product runs on the bf16 matrix cores without losing a bit of its operands.
 ``linear`` / ``Linear`` is the layer whose backward does so (float32, the framework's own products either way).
 
+``pack``, ``unpack`` and ``weight_grad`` are not recorded by autograd; ``linear`` is differentiable (once, backward() only).  Tensors with a
+forward-mode derivative are refused, and so is recording by torch.jit.trace or make_fx, which would miss the kernels.
+
 No counterpart in the reference, which keeps everything in float32.
 """
 import torch
@@ -84,6 +87,7 @@ class Packed8(object):
 def pack(x, relu=False):
     """The 8-bit checkpoint of ``x`` [..., cols], or of max(x, 0) with ``relu``."""
     relu = bool(relu)
+    L.no_tangents("pack", x)
     return Packed8._of(kernels.backend().act8_pack(_as_rows(x, "pack: x"), relu), x.shape, relu, x.dtype)
 
 
@@ -94,6 +98,7 @@ def weight_grad(dy, packed, bias=True):
     if not isinstance(packed, Packed8):
         raise RuntimeError("weight_grad: packed must be a Packed8 (got %s)" % type(packed).__name__)
     dy2 = _as_rows(dy, "weight_grad: dy")
+    L.no_tangents("weight_grad", dy)
     if dy.shape[:-1] != packed.shape[:-1] or dy.get_device() != packed.codes.get_device():
         raise RuntimeError("weight_grad: dy %s on %s does not belong to a checkpoint of %s on %s"
                            % (tuple(dy.shape), dy.device, packed.shape, packed.codes.device))
@@ -151,6 +156,7 @@ def linear(x, weight, bias=None, packed=None):
         raise RuntimeError("linear: bias %s does not go with weight %s" % (tuple(bias.shape), tuple(weight.shape)))
     if packed is not None and (not isinstance(packed, Packed8) or packed.shape != tuple(x.shape) or packed.codes.device != x.device):
         raise RuntimeError("linear: packed is not a checkpoint of x %s" % (tuple(x.shape),))
+    L.no_tangents("linear", x, weight, bias)
     # (needs_input_grad does not know of no_grad: a prediction would pack what nothing reads)
     keep = torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad))
     return _Linear8.apply(x, weight, bias, packed, keep)

@@ -10,7 +10,8 @@
 ``bits=8`` keeps z for the backward as an 8-bit checkpoint (dun_amd.act8): xhat is then taken from the checkpoint's values and the
 forward's mean and rstd.  float32, bfloat16 and float16 rows; statistics and sums in float32; weight and bias of any of these types.
 
-``layer_norm`` is differentiable (once); ``layer_norm_forward`` / ``layer_norm_backward`` are the two halves for callers
+``layer_norm`` is differentiable (once, backward() only: tensors with a forward-mode derivative are refused, and so is recording by
+torch.jit.trace or make_fx, which would miss the kernels); ``layer_norm_forward`` / ``layer_norm_backward`` are the two halves for callers
 that run their backward themselves, like the trunks of this package.  Both can be captured into a HIP graph.  A captured
 ``backward()`` goes by torch's rule for every operator: no earlier autograd graph of the same leaves may be alive (its
 gradient accumulators belong to another stream, which ends the process); the two halves have none.  Batches couple nowhere: no running statistics, no
@@ -22,6 +23,7 @@ import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
+from . import _lib as L
 from . import kernels
 from .act8 import Packed8, _as_rows
 
@@ -41,6 +43,7 @@ def _vector(t, cols, x, what):
 
 def _checked(x, weight, bias, eps, residual, bits):
     x2 = _as_rows(x, "layer_norm: x")
+    L.no_tangents("layer_norm", x, weight, bias, residual)
     cols = x2.shape[1]
     w = None if weight is None else _vector(weight, cols, x, "weight")
     b = None if bias is None else _vector(bias, cols, x, "bias")
@@ -86,6 +89,7 @@ def layer_norm_backward(dy, saved, sum_dx=False, weight_grads=True):
     if dy.shape != saved.shape or dy.dtype != saved.dtype or dy.get_device() != saved.stats.get_device():
         raise RuntimeError("layer_norm_backward: dy %s %s on %s does not go with x %s %s on %s"
                            % (tuple(dy.shape), dy.dtype, dy.device, tuple(saved.shape), saved.dtype, saved.stats.device))
+    L.no_tangents("layer_norm_backward", dy)
     dy2 = dy if dy.dim() == 2 else dy.reshape(-1, dy.shape[-1])
     dx, sums = kernels.backend().layer_norm_backward(dy2, saved.x, saved.packed, saved.w, saved.stats, saved.relu,
                                                      3 if sum_dx else 2 if weight_grads else 0)
