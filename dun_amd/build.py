@@ -16,6 +16,10 @@ LIB = os.path.join(HERE, "libdun_hip.so")
 SOURCES = ["api.hip", "gemm.hip", "elbo.hip", "head.hip", "trunk.hip", "smallnet.hip", "persist.hip",
            "norm.hip", "act8.hip"]
 ARCH = "gfx950"
+# packed fp32 instructions off: some of their forms have given wrong results on this hardware now and then (the host
+# pass warns that it does not know the feature)
+FLAGS = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
@@ -38,18 +42,14 @@ def build_library(force=False, verbose=False):
                os.path.join(CSRC, "rows.h"), os.path.join(HERE, "..", "include", "dun_hip.h")]
     objdir = os.path.join(HERE, "build")
     os.makedirs(objdir, exist_ok=True)
-    # packed fp32 instructions off: some of their forms have given wrong results on this hardware now and then (the host
-    # pass warns that it does not know the feature)
-    flags = ["--offload-arch=" + ARCH, "-O3", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
-             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     jobs = []
     objs = []
     for src in SOURCES:
         s = os.path.join(CSRC, src)
         o = os.path.join(objdir, src.replace(".hip", ".o"))
         objs.append(o)
-        if force or _stale(o, [s] + headers):
-            jobs.append([hipcc] + flags + ["-c", s, "-o", o])
+        if force or _stale(o, [s, os.path.abspath(__file__)] + headers):  # (this file: the flags)
+            jobs.append([hipcc] + FLAGS + ["-c", s, "-o", o])
 
     def run(cmd):
         if verbose:

@@ -15,7 +15,7 @@ if "--build" in sys.argv:
     B.build_library()
     objdir = os.path.join(ROOT, "dun_amd", "build")
     o = os.path.join(objdir, "gemm_timing%s.o" % TAG)
-    subprocess.run([B._hipcc(), "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-DDUN_GEMM_TIMING"] +
+    subprocess.run([B._hipcc()] + B.FLAGS + ["-DDUN_GEMM_TIMING"] +
                    os.environ.get("DUN_TIMING_FLAGS", "").split() + ["-c",
                     os.path.join(B.CSRC, "gemm.hip"), "-o", o], check=True)
     objs = [os.path.join(objdir, s.replace(".hip", ".o")) for s in B.SOURCES if s != "gemm.hip"] + [o]
