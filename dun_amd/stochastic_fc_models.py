@@ -432,7 +432,11 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
             be.head_forward(buf.h(0), p["w_out"], p["b_out"], out=buf.act[0])
         for i in range(depth):
             h, z = buf.h(i), buf.z(i)
-            be.gemm(h, p["w"][i], B, W, W, bias=p["b"][i], relu=True, out=z)
+            be.gemm(h, p["w"][i], B, W, W, bias=p["b"][i], out=z)
+            # Rectified by the norm that reads it, which keeps NaN: the product's own ReLU makes a NaN 0, and a diverged weight would
+            # not show.  The float32 planes that training keeps hold it rectified: a pass in place, 0.2 ms at 65536 x 2048.
+            if buf.keep32:
+                z.relu_()
             be.layer_norm_forward(z, p["gamma"][i], p["beta"][i], self.ln_eps, res=h, relu=True, want_stats=train,
                                   stats=buf.stats[i] if train else None, out=buf.h(i + 1), pack_x=buf.keep8, pack_y=buf.keep8,
                                   x_packed=buf.rows8(buf.Zq, i), y_packed=buf.rows8(buf.Hq, i + 1))

@@ -186,3 +186,20 @@ def test_a_capture_beside_an_older_graph_is_refused():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(held.detach(), m(x).detach())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("train", [True, False])
+def test_a_diverged_weight_shows(dev, bits, train):
+    """A NaN that a block's Linear makes is a NaN behind the block's ReLU, as torch's is: in every row from that depth on, and in the gradients."""
+    m = build(dev, bits).model.train(train)
+    with torch.no_grad():
+        m.stochstic_layers[1].block[0].weight[3, 7] = float("nan")
+    x = torch.randn(33, 5, device=dev)
+    act = m(x)
+    assert torch.isfinite(act[:2]).all() and torch.isnan(act[2:]).all()
+    if train and (dev == "cuda" or bits == 32):  # (the CPU stand-in's checkpoints read a group without numbers back as zeros)
+        act.backward(torch.ones_like(act))
+        for n, p in m.named_parameters():
+            if not n.startswith("stochstic_layers.2") and n not in ("output_layer.bias", "stochstic_layers.1.block.2.bias"):
+                assert torch.isnan(p.grad).any(), n
