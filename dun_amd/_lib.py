@@ -33,6 +33,7 @@ EXPORTS = [
 SGD_MAX_SEGMENTS = 24
 ROW_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DUN_F32, DUN_BF16, DUN_F16
 ACT8_GROUP = 32
+ROW_MOST = 2 ** 31 - 1 - 65536  # elements a row: the entries' 32-bit column counts, with room for a kernel's step
 
 
 def res_floats(D):

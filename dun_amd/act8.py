@@ -40,6 +40,8 @@ def _as_rows(t, what):
             t = t.reshape(-1, t.shape[-1])
     if t.shape[-1] == 0:
         raise RuntimeError("%s has rows of no elements: %s" % (what, tuple(t.shape)))
+    if t.shape[-1] > L.ROW_MOST:
+        raise RuntimeError("%s has more than %d elements a row: %s" % (what, L.ROW_MOST, tuple(t.shape)))
     return t
 
 
@@ -152,6 +154,8 @@ def linear(x, weight, bias=None, packed=None):
             raise RuntimeError("linear: %s must be float32 on %s (got %s on %s)" % (what, x.device, t.dtype, t.device))
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
         raise RuntimeError("linear: x %s does not go with weight %s" % (tuple(x.shape), tuple(weight.shape)))
+    if x.numel() // x.shape[-1] >= 1 << 31 or max(weight.shape) >= 1 << 31:
+        raise RuntimeError("linear: x %s and weight %s: at most 2^31 - 1 rows, inputs and outputs" % (tuple(x.shape), tuple(weight.shape)))
     if bias is not None and tuple(bias.shape) != (weight.shape[0],):
         raise RuntimeError("linear: bias %s does not go with weight %s" % (tuple(bias.shape), tuple(weight.shape)))
     if packed is not None and (not isinstance(packed, Packed8) or packed.shape != tuple(x.shape) or packed.codes.device != x.device):
