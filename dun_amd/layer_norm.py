@@ -96,10 +96,10 @@ def layer_norm_backward(dy, saved, sum_dx=False, weight_grads=True):
     if sums is None:
         return dx if dy.dim() == 2 else dx.view(saved.shape), None, None
     rows = sums.unbind(0)
-    dw, db = rows[0], rows[1]
-    if saved.w_dtype not in (None, torch.float32):
+    dw, db = (rows[0], rows[1]) if weight_grads else (None, None)
+    if weight_grads and saved.w_dtype not in (None, torch.float32):
         dw = dw.to(saved.w_dtype)
-    if saved.b_dtype not in (None, torch.float32):
+    if weight_grads and saved.b_dtype not in (None, torch.float32):
         db = db.to(saved.b_dtype)
     dx = dx if dy.dim() == 2 else dx.view(saved.shape)
     return (dx, dw, db, rows[2]) if sum_dx else (dx, dw, db)

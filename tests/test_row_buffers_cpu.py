@@ -157,3 +157,13 @@ def test_supplied_buffers_of_another_type_are_refused(entries):
     for kw in (dict(dw=half(8, 8)), dict(db=half(8))):
         with pytest.raises(RuntimeError, match="float32"):
             be.act8_weight_grad(dy, packed, 8, False, **kw)
+
+
+def test_weight_gradients_are_none_where_they_are_not_asked_for(entries):
+    x = torch.zeros(6, 40)
+    entries.hold(x)
+    _, saved = layer_norm_forward(x)
+    assert layer_norm_backward(x, saved, weight_grads=False)[1:] == (None, None)
+    dx, dw, db, ds = layer_norm_backward(x, saved, sum_dx=True, weight_grads=False)
+    assert dw is None and db is None and ds.shape == (40,)
+    assert all(t is not None for t in layer_norm_backward(x, saved, sum_dx=True))
