@@ -218,6 +218,8 @@ def out_ptr(t):
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_tracing = torch._C._get_tracing_state
+_modes = torch._C._len_torch_dispatch_stack
 
 
 def gpu_index(t):
@@ -225,7 +227,7 @@ def gpu_index(t):
     i = t.get_device()
     if i < 0:
         raise RuntimeError("dun_amd kernels need GPU tensors (got a %s tensor); there is no CPU path" % t.device)
-    if torch._C._get_tracing_state() is not None or (torch._C._len_torch_dispatch_stack() and _recorded()):
+    if _tracing() is not None or (_modes() and _recorded()):
         # (a recording would hold the allocation of the output and not the kernel that fills it)
         raise RuntimeError("dun_amd kernels are not operators of a recorded graph (torch.jit.trace, make_fx); capture a HIP graph")
     return i
@@ -237,8 +239,9 @@ def _recorded():
 
 
 def no_tangents(what, *tensors):
-    """Refuses tensors that carry a forward-mode derivative: the kernels have none, and the result would look like a constant."""
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    """Refuses tensors that carry a forward-mode derivative: the kernels have none, and the result would look like a constant.  (There are
+    none outside forward_ad.dual_level: callers ask for forward_ad._current_level >= 0 first.)"""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError("%s has no forward-mode derivative (backward() only)" % what)
 
 

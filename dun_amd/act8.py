@@ -21,6 +21,7 @@ No counterpart in the reference, which keeps everything in float32.
 """
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -38,9 +39,10 @@ def _as_rows(t, what):
             raise RuntimeError("%s must be a tensor of at least one dimension" % what)
         if t.shape[-1]:
             t = t.reshape(-1, t.shape[-1])
-    if t.shape[-1] == 0:
-        raise RuntimeError("%s has rows of no elements: %s" % (what, tuple(t.shape)))
-    if t.shape[-1] > L.ROW_MOST:
+    cols = t.shape[-1]
+    if not 0 < cols <= L.ROW_MOST:
+        if cols == 0:
+            raise RuntimeError("%s has rows of no elements: %s" % (what, tuple(t.shape)))
         raise RuntimeError("%s has more than %d elements a row: %s" % (what, L.ROW_MOST, tuple(t.shape)))
     return t
 
@@ -89,7 +91,8 @@ class Packed8(object):
 def pack(x, relu=False):
     """The 8-bit checkpoint of ``x`` [..., cols], or of max(x, 0) with ``relu``."""
     relu = bool(relu)
-    L.no_tangents("pack", x)
+    if forward_ad._current_level >= 0:
+        L.no_tangents("pack", x)
     return Packed8._of(kernels.backend().act8_pack(_as_rows(x, "pack: x"), relu), x.shape, relu, x.dtype)
 
 
@@ -100,7 +103,8 @@ def weight_grad(dy, packed, bias=True):
     if not isinstance(packed, Packed8):
         raise RuntimeError("weight_grad: packed must be a Packed8 (got %s)" % type(packed).__name__)
     dy2 = _as_rows(dy, "weight_grad: dy")
-    L.no_tangents("weight_grad", dy)
+    if forward_ad._current_level >= 0:
+        L.no_tangents("weight_grad", dy)
     if dy.shape[:-1] != packed.shape[:-1] or dy.get_device() != packed.codes.get_device():
         raise RuntimeError("weight_grad: dy %s on %s does not belong to a checkpoint of %s on %s"
                            % (tuple(dy.shape), dy.device, packed.shape, packed.codes.device))
@@ -160,7 +164,8 @@ def linear(x, weight, bias=None, packed=None):
         raise RuntimeError("linear: bias %s does not go with weight %s" % (tuple(bias.shape), tuple(weight.shape)))
     if packed is not None and (not isinstance(packed, Packed8) or packed.shape != tuple(x.shape) or packed.codes.device != x.device):
         raise RuntimeError("linear: packed is not a checkpoint of x %s" % (tuple(x.shape),))
-    L.no_tangents("linear", x, weight, bias)
+    if forward_ad._current_level >= 0:
+        L.no_tangents("linear", x, weight, bias)
     # (needs_input_grad does not know of no_grad: a prediction would pack what nothing reads)
     keep = torch.is_grad_enabled() and (weight.requires_grad or (bias is not None and bias.requires_grad))
     return _Linear8.apply(x, weight, bias, packed, keep)

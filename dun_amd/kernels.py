@@ -472,8 +472,8 @@ class HipBackend(object):
     # them out.  Shapes and types are the callers' business (dun_amd.layer_norm, dun_amd.act8).
     def act8_buffers(self, rows, cols, device):
         groups = (cols + L.ACT8_GROUP - 1) // L.ACT8_GROUP
-        return (torch.empty((rows, groups * L.ACT8_GROUP), device=device, dtype=torch.uint8),
-                torch.empty((rows, groups), device=device, dtype=torch.uint8))
+        codes = torch.empty((rows, groups * L.ACT8_GROUP), device=device, dtype=torch.uint8)
+        return codes, codes.new_empty((rows, groups))
 
     def act8_pack(self, x, relu, out=None):
         gpu = L.gpu_index(x)
@@ -498,7 +498,7 @@ class HipBackend(object):
             with ctx:
                 return self.act8_unpack(packed, cols, relu, dtype)
         rows = codes.shape[0]
-        out = torch.empty((rows, cols), device=codes.device, dtype=dtype)
+        out = codes.new_empty((rows, cols), dtype=dtype)
         rc = L.lib().dun_act8_unpack(codes.data_ptr(), exps.data_ptr(), out.data_ptr(), cols, rows, cols, L.ROW_DTYPES[dtype], relu,
                                      L.raw_stream(gpu))
         if rc:
@@ -518,14 +518,18 @@ class HipBackend(object):
         rows, outs = dy.shape
         if ld > 1 << 24:  # (the kernels' row stride ends there)
             dy, ld = dy.detach().contiguous(), outs
-        dt, dev = L.ROW_DTYPES[dy.dtype], dy.device
+        dt = L.ROW_DTYPES[dy.dtype]
         if dw is None:
-            dw = torch.empty((outs, cols), device=dev, dtype=torch.float32)
-        if db is None and want_bias:
-            db = torch.empty((outs,), device=dev, dtype=torch.float32)
+            dw = torch.empty((outs, cols), device=dy.device, dtype=torch.float32)
+        else:
+            L.f32(dw)
+        if db is not None:
+            L.f32(db)
+        elif want_bias:
+            db = dw.new_empty((outs,))
         n_ws = lib.dun_act8_weight_grad_workspace_floats(rows, outs, cols, dt)
-        ws = torch.empty((n_ws,), device=dev, dtype=torch.float32) if n_ws else None
-        rc = lib.dun_act8_weight_grad(dy.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), L.f32(dw), None if db is None else L.f32(db),
+        ws = dw.new_empty((n_ws,)) if n_ws else None
+        rc = lib.dun_act8_weight_grad(dy.data_ptr(), ld, codes.data_ptr(), exps.data_ptr(), dw.data_ptr(), None if db is None else db.data_ptr(),
                                       None if ws is None else ws.data_ptr(), n_ws, rows, outs, cols, dt, relu, L.raw_stream(gpu))
         if rc:
             L.check(rc, "dun_act8_weight_grad")
@@ -545,8 +549,10 @@ class HipBackend(object):
         ldr = 0
         if res is not None:
             res, ldr = L.rows_view(res)
-        y = torch.empty((rows, cols), device=x.device, dtype=x.dtype) if out is None else out
-        if want_stats and stats is None:
+        y = x.new_empty((rows, cols)) if out is None else out
+        if stats is not None:
+            L.f32(stats)
+        elif want_stats:
             stats = torch.empty((2, rows), device=x.device, dtype=torch.float32)
         xq = yq = None
         xc = xe = yc = ye = None
@@ -558,7 +564,7 @@ class HipBackend(object):
             yc, ye = yq[0].data_ptr(), yq[1].data_ptr()
         rc = L.lib().dun_layer_norm_forward(
             x.data_ptr(), ldx, None if res is None else res.data_ptr(), ldr, None if w is None else w.data_ptr(),
-            None if b is None else b.data_ptr(), y.data_ptr(), cols, None if stats is None else L.f32(stats), xc, xe, yc, ye,
+            None if b is None else b.data_ptr(), y.data_ptr(), cols, None if stats is None else stats.data_ptr(), xc, xe, yc, ye,
             rows, cols, L.ROW_DTYPES[x.dtype], eps, relu, L.raw_stream(gpu))
         if rc:
             L.check(rc, "dun_layer_norm_forward")
@@ -574,20 +580,23 @@ class HipBackend(object):
         lib = L.lib()
         dy, lddy = L.rows_view(dy)
         rows, cols = dy.shape
-        dev, dt = dy.device, L.ROW_DTYPES[dy.dtype]
+        dt = L.ROW_DTYPES[dy.dtype]
         ldx = 0
         if x is not None:
             x, ldx = L.rows_view(x)
         if dx is None:
-            dx = torch.empty((rows, cols), device=dev, dtype=dy.dtype)
-        if sums and sums_out is None:
-            sums_out = torch.empty((sums, cols), device=dev, dtype=torch.float32)
+            dx = dy.new_empty((rows, cols))
+        stats_ptr = L.f32(stats)  # (float32: what is made from it is, too)
+        if sums_out is not None:
+            L.f32(sums_out)
+        elif sums:
+            sums_out = stats.new_empty((sums, cols))
         n_ws = lib.dun_layer_norm_backward_workspace_floats(rows, cols, dt, sums)
-        ws = torch.empty((n_ws,), device=dev, dtype=torch.float32) if n_ws else None
+        ws = stats.new_empty((n_ws,)) if n_ws else None
         codes, exps = (None, None) if packed is None else (packed[0].data_ptr(), packed[1].data_ptr())
         rc = lib.dun_layer_norm_backward(
             dy.data_ptr(), lddy, None if x is None else x.data_ptr(), ldx, codes, exps, None if w is None else w.data_ptr(),
-            L.f32(stats), dx.data_ptr(), cols, None if sums_out is None else L.f32(sums_out), sums,
+            stats_ptr, dx.data_ptr(), cols, None if sums_out is None else sums_out.data_ptr(), sums,
             None if ws is None else ws.data_ptr(), n_ws, rows, cols, dt, relu, L.raw_stream(gpu))
         if rc:
             L.check(rc, "dun_layer_norm_backward")

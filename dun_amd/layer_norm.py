@@ -21,6 +21,7 @@ The reference's blocks know BatchNorm only (src/DUN/layers.py:33-53).
 """
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
@@ -43,7 +44,8 @@ def _vector(t, cols, x, what):
 
 def _checked(x, weight, bias, eps, residual, bits):
     x2 = _as_rows(x, "layer_norm: x")
-    L.no_tangents("layer_norm", x, weight, bias, residual)
+    if forward_ad._current_level >= 0:
+        L.no_tangents("layer_norm", x, weight, bias, residual)
     cols = x2.shape[1]
     w = None if weight is None else _vector(weight, cols, x, "weight")
     b = None if bias is None else _vector(bias, cols, x, "bias")
@@ -67,7 +69,7 @@ class Saved(object):
 
 def layer_norm_forward(x, weight=None, bias=None, eps=1e-5, residual=None, relu=False, bits=None, pack_output=False):
     """-> (y, saved), or (y, saved, Packed8 of y) with ``pack_output``.  Not recorded by autograd; ``saved`` refers to
-    ``x`` itself unless ``bits`` is 8: x must not change before ``layer_norm_backward``."""
+    ``weight`` itself and, unless ``bits`` is 8, to ``x``: they must not change before ``layer_norm_backward``."""
     x2, w, b, r2 = _checked(x, weight, bias, eps, residual, bits)
     relu = bool(relu)
     y, stats, xq, yq = kernels.backend().layer_norm_forward(x2, w, b, eps, r2, relu, True, bits == 8, bool(pack_output))
@@ -89,7 +91,8 @@ def layer_norm_backward(dy, saved, sum_dx=False, weight_grads=True):
     if dy.shape != saved.shape or dy.dtype != saved.dtype or dy.get_device() != saved.stats.get_device():
         raise RuntimeError("layer_norm_backward: dy %s %s on %s does not go with x %s %s on %s"
                            % (tuple(dy.shape), dy.dtype, dy.device, tuple(saved.shape), saved.dtype, saved.stats.device))
-    L.no_tangents("layer_norm_backward", dy)
+    if forward_ad._current_level >= 0:
+        L.no_tangents("layer_norm_backward", dy)
     dy2 = dy if dy.dim() == 2 else dy.reshape(-1, dy.shape[-1])
     dx, sums = kernels.backend().layer_norm_backward(dy2, saved.x, saved.packed, saved.w, saved.stats, saved.relu,
                                                      3 if sum_dx else 2 if weight_grads else 0)

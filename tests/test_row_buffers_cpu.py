@@ -17,7 +17,7 @@ def span(rows, cols, ld):
 
 
 class Entries(object):
-    """Stands for the library.  `seen`: every tensor that torch.empty made or a test registered, by its address."""
+    """Stands for the library.  `seen`: every tensor that torch.empty or new_empty made or a test registered, by its address."""
 
     def __init__(self):
         self.real, self.seen, self.calls = L.lib(), {}, []
@@ -101,14 +101,15 @@ class Entries(object):
 @pytest.fixture
 def entries(monkeypatch):
     e = Entries()
-    empty = torch.empty
+    def recorded(make):
+        def made(*args, **kw):
+            t = make(*args, **kw)
+            e.hold(t)
+            return t
+        return made
 
-    def recorded(*args, **kw):
-        t = empty(*args, **kw)
-        e.hold(t)
-        return t
-
-    monkeypatch.setattr(torch, "empty", recorded)
+    monkeypatch.setattr(torch, "empty", recorded(torch.empty))
+    monkeypatch.setattr(torch.Tensor, "new_empty", recorded(torch.Tensor.new_empty))
     monkeypatch.setattr(L, "lib", lambda: e)
     monkeypatch.setattr(L, "gpu_index", lambda t: 0)
     monkeypatch.setattr(L, "elsewhere", lambda i: None)
