@@ -1,13 +1,14 @@
 """8-bit activation checkpoints and the gradients that are taken from them.
 
-A training step keeps every layer's input for its backward.  ``pack`` keeps it in 1 + 1/32 bytes per element: 8-bit codes and one
-power-of-two scale per 32 consecutive columns of a row,
+A training step keeps every layer's input for its backward.  ``pack`` keeps it in 33 bytes per 32 consecutive columns of a row, 8-bit
+codes and one power-of-two scale (1 + 1/32 bytes an element; a row's last group counts whole: 132 bytes for 100 columns, 33 for one),
 
     value = code * 2^e,   e the smallest integer (not below -126) for which the group's largest magnitude rounds to at
                           most 127 (255 for a rectified input, ``relu=True``: unsigned codes of max(x, 0)),
 
-rounded to nearest even, so an element is off by at most half a step and a step is at most the group's largest magnitude / 63.75
-(127.75 rectified).  A positive element of a rectified input keeps a code of at least 1: ``value > 0`` is ReLU's mask.
+rounded to nearest even.  A positive element of a rectified input keeps a code of at least 1: ``value > 0`` is ReLU's mask.  So an element is off
+by at most half a step, and a positive rectified one below half a step by less than a step; a step is at most the group's largest
+magnitude / 63.75 (127.75 rectified), or 2^-126 where that is more.
 A group that holds an infinity or a NaN, or whose largest magnitude would round to 2^128, reads back as NaN.
 
 ``weight_grad`` takes a Linear layer's weight gradient straight from the codes: a value is a bf16 number, an fp32

@@ -19,7 +19,7 @@ typedef u32 u32x4_any __attribute__((ext_vector_type(4), aligned(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 
 // ---- pack / unpack: elementwise streams -----------------------------------------------------------------------------------------
-// 65536 x 2048 fp32: pack 147 us, unpack 126 us (4.6, 5.4 TB/s).
+// 65536 x 2048 fp32: pack 147 us, unpack 128 - 144 us (4.6, 4.7 - 5.3 TB/s); bf16 125 and 103 us (3.2, 3.9 TB/s).
 // One vector of E columns per lane; a row is G * 32 / E vectors (padded groups included), so the lanes of a group are neighbours.
 template <typename T>
 __global__ __launch_bounds__(256) void act8_pack_kernel(const T* x, size_t ldx, uint8_t* codes, uint8_t* exps, size_t vecs,
@@ -195,7 +195,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_buffer(const void* p, u32
 // columns per step, low.
 // 65536 x 2048 x 2048 fp32: 1.31 ms, 1.26 PFLOP/s of bf16 products (an 8192^3 bf16 product of the installed library: 1.20), the matrix pipe busy
 // for 66 % of the cycles at a clock that falls to 1.6 GHz under it.  On the way: loads under branches, waited for where they were
-// issued, 1.54 ms (49 %); an fp32 product of the library 4.2 ms.  bf16 dy 0.72 ms: one MFMA a tile, the staging shows.
+// issued, 1.54 ms (49 %); an fp32 product of the library 4.2 ms.  fp16 dy 0.93 ms (1.18 PFLOP/s), bf16 dy 0.61 ms (0.90): one MFMA a tile,
+// the staging shows.
 // A column's four 16-byte chunks (8 rows each) and the column's place among its neighbours are permuted by its
 // index so that the writes (columns 1, 2 or 4 apart, one chunk) and the reads (columns in a row, one chunk) spread over the banks.
 __device__ __forceinline__ int lds_chunk(int col, int kc) {
@@ -431,7 +432,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64, (BM / WM) * (BN / WN) >
 // rows and takes both operands from global memory straight into the MFMA's registers, no LDS: v_mfma_f32_16x16x32_bf16 wants rows
 // 8 (l / 16) .. + 7 of column l % 16 in lane l, and WHICH column of dw that is, is free: with the lane's 16 codes per row (one
 // load) being columns 16 (l % 16) + t, tile t = 0 .. 15 takes byte t of every load.  49152 x 10 x 2048: 31 us, 3.4 TB/s (without the loads of the
-// next rows under way 46 us); what is left is the latency of six steps a wave.
+// next rows under way 46 us): 48 ranges of rows x 8 column tiles are 384 workgroups on 256 CUs, and a wave has eight steps whose load
+// latency shows.  65536 x 32 x 2048, two groups: 48 us, 3.0 TB/s.
 template <typename T, bool SIGNED, int G>
 __global__ __launch_bounds__(256, 2) void act8_wgrad_narrow_kernel(const WgradP p) {
     constexpr int N = Terms<T>::N;
@@ -564,7 +566,7 @@ static void wgrad_split(WgradPlan* q, size_t rows, size_t s) {
 }
 
 // Tile and number of row ranges with the least estimated time: steps of 32 rows times what a step of that tile takes with 1, 2 or 4
-// workgroups on each of 256 CUs (measured, fp32 dy, us), times the rounds, plus the partial results, written and read, and the launch that
+// workgroups on each of 256 CUs (measured with fp32 dy, us, and taken for 16-bit ones too, whose steps are shorter), times the rounds, plus the partial results, written and read, and the launch that
 // adds them up.  Over 24 shapes from 512 x 40 x 40 to 65536 x 2048 x 100 the choice is within 9 % of the best of all tiles and splits,
 // 1.5 % on average; the large tile alone would be 1.6 times slower on the small ones (512 x 100 x 100: 17.2 us against 10.8), the
 // small one 1.5 times on the large (65536 x 100 x 2048: 202 us against 125).

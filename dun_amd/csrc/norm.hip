@@ -14,9 +14,11 @@
 // sees the same columns), added up over a workgroup in LDS in a fixed order, and over workgroups by a second small
 // kernel: no atomics, the same bits every time.
 //
-// 65536 x 2048 fp32: forward 200 us, backward 300 us, 5.4 TB/s both (a copy of 1 GiB: 5.2); the residual block with its checkpoint
-// 300 us and, from the codes, 218 us (5.8, 5.6 TB/s).  16391 x 1031 bf16, where rows start anywhere: 28 and 29 us (2.4, 3.5 TB/s): too
-// few bytes in flight, a row of 2 KB on two waves.  Small ones are launches: 512 x 100 fp32 4.2 + 4.4 + 2.7 us.
+// 65536 x 2048 fp32 (a copy of 1 GiB: 5.2 TB/s): forward 231 - 248 us by itself, 205 us in turn with a backward (4.5, 5.2 TB/s), backward 292 -
+// 300 us (5.4); the residual block with its checkpoint 300 us and, from the codes, 216 - 220 us (5.8, 5.6 TB/s), with its output packed
+// as well 356 us.  bf16, half the bytes: forward 166 - 187 us, backward 176 us, block 256 - 264 us and 176 us: 3.1 and 4.6 TB/s, four elements
+// a load whatever the type.  16391 x 1031 bf16, where rows start anywhere: 25 and 28 us (2.7, 3.6 TB/s): too few bytes in flight, a
+// row of 2 KB on two waves.  Small ones are launches: 512 x 100 fp32 3.6 + 4.2 + 2.7 us.
 #include "rows.h"
 
 namespace dun {
@@ -250,7 +252,8 @@ __global__ __launch_bounds__(ln_block<TEAM>()) void ln_backward_kernel(const LnB
     // A lane sees the same columns in every row.  Weights that stay in registers spare each row a wait for the cache:
     // with them in 16-bit rows 16391 x 1031 takes 29 us and not 38, in fp32 rows with 8-bit codes 65536 x 2048 takes
     // 218 us and not 237.  Plain fp32 rows are bound by memory and want the waves instead: 310 us at 65536 x 2048 with
-    // the weights read row by row, 338 with them kept.
+    // the weights read row by row, 338 with them kept.  The MASK forms serve codes and x alike and keep them for both: fp32 rows
+    // read from x take 320 - 324 us there (rectified, with the sums of dx, or dx alone) where the plain form takes 292.
     constexpr bool KEEP_W = MASK || sizeof(T) < 4;
     RawVec<float> w[CH];
     auto weights = [&] {
@@ -479,9 +482,10 @@ __global__ __launch_bounds__(LN_LONG_THREADS) void ln_backward_long_kernel(const
 // ---- host side ---------------------------------------------------------------------------------------------------------------
 // Teams and vectors of four elements per lane, by the elements that a team holds: the fewest lanes up to a wave, then more vectors per
 // lane, then more waves.  What decides is the bytes in flight: few registers per row for many rows at a time, but no idle lanes.
-// 65536 x 2048 fp32, forward / backward: 64 x 8 237 / 330 us, 256 x 2 200 / 297 us (a plain copy of as many bytes: 208 / 312);
-// 16391 x 1031 bf16: 256 x 2, half of its lanes idle, 34 / 60 us, 128 x 3 26 / 38 us (since: 28 / 29).  512 x 8 for rows of up to 16384 elements spills: 2000 x
-// 16384 fp32 96 / 163 us, walked in memory 75 / 235 us.
+// 65536 x 2048 fp32, forward / backward in turn: 64 x 8 237 / 330 us, 256 x 2 200 / 297 us (a plain copy of as many bytes: 208 / 312);
+// 16391 x 1031 bf16: 256 x 2, half of its lanes idle, 34 / 60 us, 128 x 3 26 / 38 us (since: 25 / 28).  512 x 8 for rows of up to 16384 elements spills: 2000 x
+// 16384 fp32 96 / 163 us, walked in memory 75 / 235 us (since: 71 / 223).  Idle lanes show between the teams: 16384 rows of 3000, 4100 and 6000
+// fp32 elements take 101 / 137, 228 / 200 and 239 / 245 us (copies of as many bytes: 76 / 114, 104 / 156, 152 / 228).
 #define DUN_LN_TEAMS(X) X(8, 1) X(16, 1) X(32, 1) X(64, 1) X(64, 2) X(64, 3) X(64, 4) X(128, 3) X(256, 2) X(256, 4) X(1024, 2)
 
 static int ln_team(int cols, int* ch) {

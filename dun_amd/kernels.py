@@ -143,7 +143,7 @@ class LnFcBuffers(object):
     """Device buffers of one LayerNorm trunk at a fixed (batch, depth, mode).
 
     Training keeps what backward reads: every block's input and rectified Linear output, in float32 (``act_bits`` 32) or as
-    8-bit checkpoints (8: 1 + 1/32 bytes an element, and one float32 hidden state that is updated in place); prediction
+    8-bit checkpoints (8: 33 bytes per 32 columns, and one float32 hidden state that is updated in place); prediction
     keeps nothing."""
 
     def __init__(self, model, B, depth, train):
