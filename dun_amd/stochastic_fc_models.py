@@ -399,8 +399,8 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
                 return super(arq_uncert_fc_resnet_ln, self).forward(x, depth, objective)
         if self._step_alone:
             return _LnFcForward.apply(self, x, self.n_layers if depth is None else depth, self.flat_params.new_empty(0).requires_grad_())
-        stream = torch.cuda.current_stream(self.flat_params.device).cuda_stream if self.flat_params.is_cuda else 0
-        if stream and torch.cuda.is_current_stream_capturing() and any(s != stream for s in list(self._nodes.values())):
+        stream = torch.cuda.current_stream(self.flat_params.device) if self.flat_params.is_cuda else None
+        if stream is not None and torch.cuda.is_current_stream_capturing() and any(s != stream for s in list(self._nodes.values())):
             raise RuntimeError("an act_vec from before this capture is still alive: its graph holds the parameters' gradient "
                                "accumulators on another stream, and a captured backward would wait for them there; drop it first")
         act = super(arq_uncert_fc_resnet_ln, self).forward(x, depth, objective)
@@ -490,3 +490,13 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
         for q, gv in zip(self._param_list, self._grad_views):
             if q.grad is not gv:
                 q.grad = gv
+        self._hold_accumulators()
+
+    def _hold_accumulators(self):
+        """A parameter's gradient accumulator runs on the stream of the oldest live graph of the parameter.  Autograd makes it wait for the
+        gradients that it adds, which may be ready before the trunk's are written, and not for those: it waits here."""
+        others = {s for s in list(self._nodes.values()) if s is not None}
+        if len(others) > 1 and not torch.cuda.is_current_stream_capturing():
+            current = torch.cuda.current_stream(self.flat_params.device)
+            for s in others - {current}:
+                s.wait_stream(current)

@@ -170,6 +170,30 @@ def test_a_captured_step_of_ones_own_with_a_penalty(bits):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kept_on", ["side", "default"])
+def test_an_older_graph_on_another_stream(kept_on):
+    """The parameters' accumulators belong to the older graph's stream; the penalty's gradients are ready before the trunk's are written (the hook
+    holds the trunk's backward back on its stream)."""
+    m = build("cuda", 8).model.train()
+    x, dact = torch.randn(33, 5, device="cuda"), torch.randn(4, 33, 1, device="cuda")
+    want = alone(m, x, dact, lambda: penalty(m))
+    default, side = torch.cuda.current_stream(), torch.cuda.Stream()
+    old, new = (side, default) if kept_on == "side" else (default, side)
+    side.wait_stream(default)
+    with torch.cuda.stream(old):
+        kept = m(x)
+    new.wait_stream(old)
+    with torch.cuda.stream(new):
+        act = m(x)
+        act.register_hook(lambda g: (torch.cuda._sleep(20_000_000), g)[1])
+        pen = penalty(m)
+        torch.autograd.backward([act, pen], [dact, torch.ones_like(pen)])
+    torch.cuda.synchronize()
+    same(m, want)
+    assert kept.grad_fn is not None
+
+
+@pytest.mark.gpu
 def test_a_capture_beside_an_older_graph_is_refused():
     m = build("cuda", 8).model.train()
     x = torch.randn(33, 5, device="cuda")
