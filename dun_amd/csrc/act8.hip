@@ -566,7 +566,8 @@ static void wgrad_split(WgradPlan* q, size_t rows, size_t s) {
 }
 
 // Tile and number of row ranges with the least estimated time: steps of 32 rows times what a step of that tile takes with 1, 2 or 4
-// workgroups on each of 256 CUs (measured with fp32 dy, us, and taken for 16-bit ones too, whose steps are shorter), times the rounds, plus the partial results, written and read, and the launch that
+// workgroups on each of 256 CUs (measured with fp32 dy, us, and taken for 16-bit ones too, whose steps are shorter), times the rounds,
+// plus the partial results, written and read, and the launch that
 // adds them up.  Over 24 shapes from 512 x 40 x 40 to 65536 x 2048 x 100 the choice is within 9 % of the best of all tiles and splits,
 // 1.5 % on average; the large tile alone would be 1.6 times slower on the small ones (512 x 100 x 100: 17.2 us against 10.8), the
 // small one 1.5 times on the large (65536 x 100 x 2048: 202 us against 125).

@@ -382,7 +382,7 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
 
     def _flatten(self):
         super(arq_uncert_fc_resnet_ln, self)._flatten()
-        if "_nodes" not in self.__dict__:  # autograd nodes of forwards that are still alive: the stream they ran on
+        if "_nodes" not in self.__dict__:  # autograd nodes of forwards that are alive: the stream of the accumulators they hold
             self._nodes = weakref.WeakKeyDictionary()
 
     def __getstate__(self):
@@ -400,11 +400,13 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
         if self._step_alone:
             return _LnFcForward.apply(self, x, self.n_layers if depth is None else depth, self.flat_params.new_empty(0).requires_grad_())
         stream = torch.cuda.current_stream(self.flat_params.device) if self.flat_params.is_cuda else None
-        if stream is not None and torch.cuda.is_current_stream_capturing() and any(s != stream for s in list(self._nodes.values())):
+        # (a live graph keeps the accumulators it found, of a graph before it perhaps, or made on its own stream)
+        home = next(iter(list(self._nodes.values())), stream)
+        if home != stream and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("an act_vec from before this capture is still alive: its graph holds the parameters' gradient "
                                "accumulators on another stream, and a captured backward would wait for them there; drop it first")
         act = super(arq_uncert_fc_resnet_ln, self).forward(x, depth, objective)
-        self._nodes[act.grad_fn] = stream
+        self._nodes[act.grad_fn] = home
         return act
 
     forward_get_acts = forward
@@ -493,10 +495,11 @@ class arq_uncert_fc_resnet_ln(arq_uncert_fc_resnet):
         self._hold_accumulators()
 
     def _hold_accumulators(self):
-        """A parameter's gradient accumulator runs on the stream of the oldest live graph of the parameter.  Autograd makes it wait for the
-        gradients that it adds, which may be ready before the trunk's are written, and not for those: it waits here."""
-        others = {s for s in list(self._nodes.values()) if s is not None}
-        if len(others) > 1 and not torch.cuda.is_current_stream_capturing():
-            current = torch.cuda.current_stream(self.flat_params.device)
-            for s in others - {current}:
-                s.wait_stream(current)
+        """A parameter's gradient accumulator runs on the stream that it was made on, by the first of the graphs that have held it since.
+        Autograd makes it wait for the gradients that it adds, which may be ready before the trunk's are written, and not for those: it
+        waits here."""
+        if not self.flat_params.is_cuda or torch.cuda.is_current_stream_capturing():
+            return
+        current = torch.cuda.current_stream(self.flat_params.device)
+        for s in set(self._nodes.values()) - {current}:
+            s.wait_stream(current)
